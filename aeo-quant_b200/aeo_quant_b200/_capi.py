@@ -15,6 +15,8 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "li
 
 BF16, F16, F32, I32, I64 = 0, 1, 2, 3, 4
 FP8_WEIGHT, FP8_ACTIVATION = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 
 _DT = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.int32: I32,
        torch.int64: I64}
@@ -84,6 +86,7 @@ _SIGS["aeoq_ep_experts_nvfp4"] = [_P, _P, _P, _L, _P, _P, _L, _L, _P, _P, _P, _I
                                   _Z, _P, _P]
 _SIGS["aeoq_ep_combine_workspace_size"] = [_I, _L, _L]
 _SIGS["aeoq_ep_combine"] = [_P, _I, _I, _P, _P, _L, _L, _P, _P, _Z, _P]
+_SIGS["aeoq_route_topk"] = [_P, _I, _L, _L, _L, _L, _I, _P, _L, _L, _I, _I, _F, _P, _P, _P]
 _RESTYPE = {"aeoq_moe_nvfp4_decode_tc_workspace_size": C.c_size_t,
             "aeoq_ep_nccl_unique_id_bytes": C.c_size_t, "aeoq_ep_dispatch_workspace_size": C.c_size_t,
             "aeoq_ep_experts_nvfp4_workspace_size": C.c_size_t, "aeoq_ep_combine_workspace_size": C.c_size_t,
@@ -158,6 +161,25 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     if major != 10:
         raise AeoqError(f"aeo_quant_b200 is built for sm_100a (B200); device {dev} is sm_{major}x")
     _SM100_DEVICES.add(dev.index)
+
+
+class _Here:
+    """The tensors' device is the current one: nothing to switch."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current: a kernel launches on the
+    current device, whichever device its pointers and stream belong to."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_ptr(device: torch.device) -> int:

@@ -1,0 +1,473 @@
+// Expert choice from router logits, one warp per token.
+//
+//   s = softmax(l) or 1 / (1 + exp(-l))            score of each expert
+//   c = s + bias, and -inf where l = -inf          what the choice goes by
+//   worth(group) = max c, or the sum of its two largest c (a missing second
+//   one counts 0); experts outside the best `topk_group` groups get c = -inf
+//   ids = the k largest c in descending order;  w = s[ids] (/ sum) * scale
+// Equal values go to the lower index. A slot for which no expert is left
+// (c = -inf) gets id E and weight 0: the expert forwards skip ids outside
+// [0, E). A row with a NaN logit or choice (softmax: or a +inf logit) gets
+// NaN weights for ids 0..k-1, so that the NaN reaches the layer's output.
+//
+// The ids are those of exact arithmetic. Without a bias both scores rise
+// with the logit, so the choice compares the logits themselves (softmax
+// probabilities of one row, and sigmoids, order as their logits do; group
+// maxima too). With a bias, or with top-2 group sums, the warp compares f32
+// values and notes whether any comparison that decided was closer than
+// their error bound; such a row (about one in a thousand at 256 experts and
+// normal logits) is done again in 64 bits.
+//
+// Layout: lane L holds the experts L*PER .. L*PER+PER-1, so a row is read
+// with wide loads and the lowest lane that holds a maximum also holds the
+// lowest index. Per choice: the lane's maximum of PER keys, one redux.sync,
+// one ballot.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace aeoq {
+
+constexpr int kRouteWarps = 4;        // rows per block
+constexpr int kRouteMaxExperts = 1024;
+constexpr int kRouteMaxK = 32;
+constexpr int kRouteMaxGroups = 32;
+
+struct RouteParams {
+  const void* logits;
+  int64_t ld, T;
+  int E, k;
+  const float* bias;     // null: none
+  int n_group, topk_group;
+  int sigmoid, top2, renorm;
+  int vec;               // rows may be read in PER-wide pieces
+  float scale;
+  float* w;
+  int64_t* ids;
+};
+
+// Floats as unsigned integers of the same order; -inf is 0x007FFFFF, so 0 is
+// free for "no such expert, or already taken".
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float order_val(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+constexpr uint32_t kNegInfKey = 0x007FFFFFu;
+
+__device__ __forceinline__ uint64_t order_key64(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  return (b >> 63) ? ~b : (b | (1ull << 63));
+}
+__device__ __forceinline__ double order_val64(uint64_t k) {
+  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
+}
+constexpr uint64_t kNegInfKey64 = 0x000FFFFFFFFFFFFFull;
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t u = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    v = u > v ? u : v;
+  }
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ float route_logit(const RouteParams& p, int64_t row, int e) {
+  return In<DT>::load(reinterpret_cast<const typename In<DT>::T*>(p.logits) + row * p.ld + e);
+}
+
+// Which groups stay: bit g of the result. top1/top2 of the groups come as the
+// (ordered) keys of lane g. `near` is set where a kept and a dropped group
+// are within tol of one another.
+template <class Val>
+__device__ __forceinline__ uint32_t keep_groups(Val worth, int n_group, int topk_group, Val tol, bool& near) {
+  const int lane = threadIdx.x & 31;
+  int rank = 0;
+  for (int h = 0; h < n_group; ++h) {
+    const Val o = __shfl_sync(0xFFFFFFFFu, worth, h);
+    rank += (o > worth) || (o == worth && h < lane);
+  }
+  const uint32_t keep = __ballot_sync(0xFFFFFFFFu, lane < n_group && rank < topk_group);
+  bool mine = false;
+  for (int h = 0; h < n_group; ++h) {
+    const Val o = __shfl_sync(0xFFFFFFFFu, worth, h);
+    const Val d = o > worth ? o - worth : worth - o;       // inf - inf is NaN: not near
+    mine |= lane < n_group && (((keep >> h) ^ (keep >> lane)) & 1u) && d <= tol;
+  }
+  near = __any_sync(0xFFFFFFFFu, mine);
+  return keep;
+}
+
+// One row in 64 bits: the same definition, plainly. Rows come here when f32
+// cannot tell two choices apart, or when every chosen score is so small that
+// f32 has lost it.
+template <int PER, int DT, bool ONLY_LOGITS>
+__device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  double s[PER];
+  uint64_t key[PER];
+  double m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane * PER + i;
+    s[i] = e < p.E ? (double)route_logit<DT>(p, row, e) : -INFINITY;
+    m = fmax(m, s[i]);
+  }
+  double total = 1.0;
+  if (!p.sigmoid) {
+    m = order_val64(warp_max64(order_key64(m)));
+    if (m == -INFINITY) m = 0.0;
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) t += exp(s[i] - m);
+    total = warp_sum64(t);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane * PER + i;
+    const double l = s[i];
+    s[i] = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : (total > 0.0 ? exp(l - m) / total : 0.0);
+    const double c = ONLY_LOGITS || l == -INFINITY ? l : s[i] + (p.bias && e < p.E ? (double)p.bias[e] : 0.0);
+    key[i] = e < p.E ? order_key64(c + 0.0) : 0ull;
+  }
+  if (p.n_group > 1) {
+    const int S = p.E / p.n_group;
+    double worth = -INFINITY;
+    for (int g = 0; g < p.n_group; ++g) {
+      uint64_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = lane * PER + i;
+        if (e >= g * S && e < (g + 1) * S) {
+          if (key[i] > a) { b = a; a = key[i]; }
+          else if (key[i] > b) b = key[i];
+        }
+      }
+      const uint64_t ga = warp_max64(a);
+      const int who = __ffs(__ballot_sync(0xFFFFFFFFu, a == ga)) - 1;
+      const uint64_t gb = warp_max64(lane == who ? b : a);
+      double v = order_val64(ga);
+      if (p.top2 && gb > kNegInfKey64) v += order_val64(gb);
+      if (lane == g) worth = v;
+    }
+    bool near;
+    const uint32_t keep = keep_groups<double>(worth, p.n_group, p.topk_group, 0.0, near);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane * PER + i;
+      if (e < p.E && !((keep >> (e / S)) & 1u)) key[i] = kNegInfKey64;
+    }
+  }
+  double my_w = 0.0;
+  int my_id = p.E;
+  for (int j = 0; j < p.k; ++j) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
+    const uint64_t top = warp_max64(best);
+    if (top <= kNegInfKey64) break;
+    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+    int at = 0;
+    double sv = 0.0;
+    if (lane == src) {
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (!done && key[i] == top) {
+          done = true;
+          key[i] = 0;
+          at = lane * PER + i;
+          sv = s[i];
+        }
+    }
+    at = __shfl_sync(0xFFFFFFFFu, at, src);
+    sv = __shfl_sync(0xFFFFFFFFu, sv, src);
+    if (lane == j) { my_id = at; my_w = sv; }
+  }
+  if (p.renorm) {
+    const double t = warp_sum64(my_w);
+    my_w = t > 0.0 ? my_w / t : 0.0;
+  }
+  if (lane < p.k) {
+    p.w[row * p.k + lane] = (float)(my_w * (double)p.scale);
+    p.ids[row * p.k + lane] = my_id;
+  }
+}
+
+// ONLY_LOGITS: no bias and no top-2 group sums, so logits decide (exactly).
+template <int PER, int DT, bool ONLY_LOGITS>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const RouteParams p) {
+  const int64_t row = blockIdx.x * (int64_t)kRouteWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= p.T) return;
+  float l[PER];
+  {
+    using Tp = typename In<DT>::T;
+    const Tp* src = reinterpret_cast<const Tp*>(p.logits) + row * p.ld + lane * PER;
+    if (p.vec) {
+      // E % PER == 0: a lane's piece lies inside the row or past it
+      constexpr int kBytes = PER * (int)sizeof(Tp);
+      __align__(16) Tp v[PER];
+      if (lane * PER < p.E) {
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+          for (int i = 0; i < kBytes / 16; ++i)
+            reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        } else if constexpr (kBytes == 8) {
+          *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(src));
+        } else if constexpr (kBytes == 4) {
+          *reinterpret_cast<uint32_t*>(v) = __ldg(reinterpret_cast<const uint32_t*>(src));
+        } else {
+          v[0] = *src;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) l[i] = In<DT>::to_f(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) l[i] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) l[i] = lane * PER + i < p.E ? In<DT>::load(src + i) : -INFINITY;
+    }
+  }
+
+  // scores
+  float s[PER];
+  bool bad = false;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    bad |= l[i] != l[i];
+    m = fmaxf(m, l[i]);
+  }
+  m = order_val(__reduce_max_sync(0xFFFFFFFFu, order_key(m)));
+  float smax;
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = __fdividef(1.0f, 1.0f + expf(-l[i]));   // 0 from a divisor of 2^126 on
+    smax = 1.0f;
+  } else {
+    bad |= m == INFINITY;
+    const float base = m == -INFINITY ? 0.0f : m;
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] = expf(l[i] - base);
+      t += s[i];
+    }
+    t = warp_sum(t);
+    const float inv = t > 0.0f ? __fdividef(1.0f, t) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] *= inv;
+    smax = inv;
+  }
+
+  // choice keys
+  uint32_t key[PER];
+  float cmax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane * PER + i;
+    float c = l[i];
+    if constexpr (!ONLY_LOGITS) {
+      const float b = (p.bias && e < p.E) ? __ldg(p.bias + e) : 0.0f;
+      c = l[i] == -INFINITY ? -INFINITY : s[i] + b;
+      bad |= c != c;
+      if (fabsf(c) < INFINITY) cmax = fmaxf(cmax, fabsf(c));
+    }
+    c += 0.0f;   // -0 and +0 are equal
+    key[i] = e < p.E ? order_key(c) : 0u;
+  }
+  if (__any_sync(0xFFFFFFFFu, bad)) {
+    if (lane < p.k) {
+      p.w[row * p.k + lane] = __int_as_float(0x7FC00000);
+      p.ids[row * p.k + lane] = lane;
+    }
+    return;
+  }
+  // How far two f32 choice values may be from the exact ones together. A
+  // softmax score: expf 2 ulp, its argument's rounding (|x| 2^-24 exp(x) <=
+  // 2^-24 / e), a sum of at most 1024 terms in chains of 37 additions and the
+  // quotient: under 3e-6 of the score. A sigmoid: under 1e-6. Then the
+  // addition of the bias, 2^-24 of the sum, twice for a group's two terms.
+  float tol = 0.0f;
+  bool again = false;
+  if constexpr (!ONLY_LOGITS) {
+    cmax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(cmax)));
+    tol = (p.sigmoid ? 2e-6f : 6e-6f) * smax + 2.5e-7f * cmax;
+  }
+
+  if (p.n_group > 1) {
+    const int S = p.E / p.n_group;
+    float worth = -INFINITY;
+    for (int g = 0; g < p.n_group; ++g) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = lane * PER + i;
+        if (e >= g * S && e < (g + 1) * S) {
+          b = max(b, min(a, key[i]));
+          a = max(a, key[i]);
+        }
+      }
+      const uint32_t ga = __reduce_max_sync(0xFFFFFFFFu, a);
+      float v = order_val(ga);
+      if (p.top2) {
+        const int who = __ffs(__ballot_sync(0xFFFFFFFFu, a == ga)) - 1;
+        const uint32_t gb = __reduce_max_sync(0xFFFFFFFFu, lane == who ? b : a);
+        if (gb > kNegInfKey) v += order_val(gb);
+      }
+      if (lane == g) worth = v;
+    }
+    bool near = false;
+    const uint32_t keep = keep_groups<float>(worth, p.n_group, p.topk_group, 2.0f * tol, near);
+    if (!ONLY_LOGITS) again = near;
+    // a lane's experts lie in at most ceil(PER / S) + 1 groups
+    int g = lane * PER / S, left = (g + 1) * S - lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (lane * PER + i < p.E && !((keep >> g) & 1u)) key[i] = kNegInfKey;
+      if (--left == 0) { ++g; left = S; }
+    }
+  }
+
+  float my_w = 0.0f;
+  int my_id = p.E;
+  float prev = INFINITY;
+  int prev_id = -1;
+  // one more round than k where the last kept and the first dropped value
+  // have to be told apart
+  const int rounds = ONLY_LOGITS ? p.k : p.k + 1;
+  for (int j = 0; j < rounds; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = max(best, key[i]);
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+    if (top <= kNegInfKey) break;
+    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+    int at = 0;
+    float sv = 0.0f;
+    if (lane == src) {
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (!done && key[i] == top) {
+          done = true;
+          key[i] = 0;
+          at = lane * PER + i;
+          sv = s[i];
+        }
+    }
+    at = __shfl_sync(0xFFFFFFFFu, at, src);
+    sv = __shfl_sync(0xFFFFFFFFu, sv, src);
+    if constexpr (!ONLY_LOGITS) {
+      const float c = order_val(top);
+      if (prev - c <= tol && prev_id >= 0) {
+        // equal logits and biases are equal in exact arithmetic too
+        const float la = route_logit<DT>(p, row, at), lb = route_logit<DT>(p, row, prev_id);
+        const float ba = p.bias ? p.bias[at] : 0.0f, bb = p.bias ? p.bias[prev_id] : 0.0f;
+        again |= !(la == lb && ba == bb);
+      }
+      prev = c;
+      prev_id = at;
+    }
+    if (lane == j && j < p.k) { my_id = at; my_w = sv; }
+  }
+  // scores that f32 holds with fewer bits, or not at all
+  const uint32_t used = __ballot_sync(0xFFFFFFFFu, my_id < p.E);
+  const float sum = warp_sum(my_w);
+  again |= used != 0 && sum < 1e-30f;
+  if (again) {
+    route_row64<PER, DT, ONLY_LOGITS>(p, row);
+    return;
+  }
+  if (p.renorm) my_w = sum > 0.0f ? my_w / sum : 0.0f;
+  if (lane < p.k) {
+    p.w[row * p.k + lane] = my_w * p.scale;
+    p.ids[row * p.k + lane] = my_id;
+  }
+}
+
+template <int PER, int DT>
+static int launch_route(const RouteParams& p, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((p.T + kRouteWarps - 1) / kRouteWarps);
+  if (!p.bias && !(p.n_group > 1 && p.top2))
+    route_topk_kernel<PER, DT, true><<<blocks, 32 * kRouteWarps, 0, st>>>(p);
+  else
+    route_topk_kernel<PER, DT, false><<<blocks, 32 * kRouteWarps, 0, st>>>(p);
+  return check_launch("route_topk_kernel");
+}
+
+template <int DT>
+static int dispatch_route(RouteParams p, cudaStream_t st) {
+  int per = 1;
+  while (per * 32 < p.E) per *= 2;
+  const int bytes = per * (int)sizeof(typename In<DT>::T), width = std::min(bytes, 16);
+  p.vec = p.E % per == 0 && (uintptr_t)p.logits % width == 0 &&
+          (p.ld * (int64_t)sizeof(typename In<DT>::T)) % width == 0;
+  switch (per) {
+    case 1: return launch_route<1, DT>(p, st);
+    case 2: return launch_route<2, DT>(p, st);
+    case 4: return launch_route<4, DT>(p, st);
+    case 8: return launch_route<8, DT>(p, st);
+    case 16: return launch_route<16, DT>(p, st);
+    default: return launch_route<32, DT>(p, st);
+  }
+}
+
+}  // namespace aeoq
+
+using namespace aeoq;
+
+extern "C" int aeoq_route_topk(const void* logits, int dtype, int64_t ld, int64_t T, int64_t num_experts, int64_t k,
+                               int score, const float* bias, int64_t n_group, int64_t topk_group, int group_score,
+                               int renormalize, float scale, float* weights, int64_t* ids, void* stream) {
+  AEOQ_REQUIRE(num_experts >= 1 && num_experts <= kRouteMaxExperts, AEOQ_ERR_INVALID,
+               "route_topk: num_experts (%lld) must be in [1, %d]", (long long)num_experts, kRouteMaxExperts);
+  AEOQ_REQUIRE(k >= 1 && k <= std::min<int64_t>(num_experts, kRouteMaxK), AEOQ_ERR_INVALID,
+               "route_topk: k (%lld) must be in [1, min(num_experts, %d)]", (long long)k, kRouteMaxK);
+  AEOQ_REQUIRE(n_group >= 1 && n_group <= kRouteMaxGroups && num_experts % n_group == 0, AEOQ_ERR_INVALID,
+               "route_topk: n_group (%lld) must be in [1, %d] and divide num_experts (%lld)", (long long)n_group,
+               kRouteMaxGroups, (long long)num_experts);
+  AEOQ_REQUIRE(topk_group >= 1 && topk_group <= n_group, AEOQ_ERR_INVALID,
+               "route_topk: topk_group (%lld) must be in [1, n_group]", (long long)topk_group);
+  AEOQ_REQUIRE((score == AEOQ_SCORE_SOFTMAX || score == AEOQ_SCORE_SIGMOID) &&
+                   (group_score == AEOQ_GROUP_MAX || group_score == AEOQ_GROUP_TOP2),
+               AEOQ_ERR_INVALID, "route_topk: bad score (%d) or group score (%d)", score, group_score);
+  AEOQ_REQUIRE(T >= 0 && ld >= num_experts, AEOQ_ERR_INVALID, "route_topk: bad shape");
+  AEOQ_REQUIRE(T <= 8LL * 1024 * 1024 * 1024, AEOQ_ERR_INVALID, "route_topk: too many tokens");
+  if (T == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(logits && weights && ids, AEOQ_ERR_INVALID, "route_topk: null pointer");
+  RouteParams p{};
+  p.logits = logits;
+  p.ld = ld;
+  p.T = T;
+  p.E = (int)num_experts;
+  p.k = (int)k;
+  p.bias = bias;
+  p.n_group = (int)(topk_group == n_group ? 1 : n_group);   // every group stays: none to choose
+  p.topk_group = (int)topk_group;
+  p.sigmoid = score == AEOQ_SCORE_SIGMOID;
+  p.top2 = group_score == AEOQ_GROUP_TOP2;
+  p.renorm = renormalize != 0;
+  p.scale = scale;
+  p.w = weights;
+  p.ids = ids;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case AEOQ_BF16: return dispatch_route<AEOQ_BF16>(p, st);
+    case AEOQ_F16: return dispatch_route<AEOQ_F16>(p, st);
+    case AEOQ_F32: return dispatch_route<AEOQ_F32>(p, st);
+  }
+  return set_error(AEOQ_ERR_INVALID, "route_topk: unsupported dtype %d", dtype);
+}

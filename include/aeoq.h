@@ -47,6 +47,12 @@ extern "C" {
 #define AEOQ_FP8_WEIGHT 0     /* quant.py:51-106 — bf16 scale per row */
 #define AEOQ_FP8_ACTIVATION 1 /* bridges/gemma4/modeling.py:101-104 — f32 scale */
 
+/* aeoq_route_topk: score of an expert, and worth of a group of experts */
+#define AEOQ_SCORE_SOFTMAX 0
+#define AEOQ_SCORE_SIGMOID 1
+#define AEOQ_GROUP_MAX 0  /* the largest choice value of the group */
+#define AEOQ_GROUP_TOP2 1 /* the sum of its two largest */
+
 /* Library version (major*10000 + minor*100 + patch). */
 AEOQ_API int aeoq_version(void);
 
@@ -469,6 +475,25 @@ AEOQ_API int aeoq_moe_nvfp4_decode_fused_noalloc(const void* hidden, const void*
                                                  const void* down_ts, int down_ts_dtype,
                                                  int64_t num_experts, int64_t hidden_dim, int64_t inter_dim,
                                                  void* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Expert choice from router logits (any MoE router whose projection is done;
+ * the Gemma-4 router above fuses its own). No counterpart in the reference.
+ *
+ * logits   T rows of num_experts values of `dtype` (BF16/F16/F32), row
+ *          stride `ld` elements.
+ * s = softmax(l) or sigmoid(l);  c = s + bias[e] (bias: f32 or null), and
+ * c = -inf where l = -inf. With n_group > 1 the experts form n_group equal
+ * runs, of which the topk_group with the largest worth stay. weights (T, k)
+ * f32 = s[ids] (divided by their sum if `renormalize`) * scale; ids (T, k)
+ * int64: the k largest c in descending order, equal values to the lower
+ * index. A slot for which no expert is left has id num_experts and weight 0;
+ * a row with a NaN (softmax: or a +inf) has NaN weights and ids 0..k-1.
+ * num_experts <= 1024, k <= 32, n_group <= 32 and dividing num_experts.
+ * ------------------------------------------------------------------------ */
+AEOQ_API int aeoq_route_topk(const void* logits, int dtype, int64_t ld, int64_t T, int64_t num_experts, int64_t k,
+                             int score, const float* bias, int64_t n_group, int64_t topk_group, int group_score,
+                             int renormalize, float scale, float* weights, int64_t* ids, void* stream);
 
 /* ------------------------------------------------------------------------
  * Self-test of the device division every quantized bit depends on: counts
