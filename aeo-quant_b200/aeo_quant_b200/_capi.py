@@ -17,6 +17,7 @@ BF16, F16, F32, I32, I64 = 0, 1, 2, 3, 4
 FP8_WEIGHT, FP8_ACTIVATION = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
+ACT_GELU_TANH, ACT_SILU = 0, 1
 
 _DT = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.int32: I32,
        torch.int64: I64}
@@ -87,7 +88,16 @@ _SIGS["aeoq_ep_experts_nvfp4"] = [_P, _P, _P, _L, _P, _P, _L, _L, _P, _P, _P, _I
 _SIGS["aeoq_ep_combine_workspace_size"] = [_I, _L, _L]
 _SIGS["aeoq_ep_combine"] = [_P, _I, _I, _P, _P, _L, _L, _P, _P, _Z, _P]
 _SIGS["aeoq_route_topk"] = [_P, _I, _L, _L, _L, _L, _I, _P, _L, _L, _I, _I, _F, _P, _P, _P]
-_RESTYPE = {"aeoq_moe_nvfp4_decode_tc_workspace_size": C.c_size_t,
+_SIGS["aeoq_fp8_block_quantize_rows"] = [_P, _I, _L, _L, _L, _P, _L, _P, _P]
+_SIGS["aeoq_fp8_block_quantize_weights"] = [_P, _I, _L, _L, _L, _P, _P, _P]
+_SIGS["aeoq_fp8_block_gemm"] = [_P, _P, _L, _P, _P, _L, _L, _P, _P, _I, _L, _P, _P]
+_SIGS["aeoq_fp8_block_linear_workspace_size"] = [_L, _L, _L]
+_SIGS["aeoq_fp8_block_linear"] = [_P, _I, _L, _L, _P, _P, _L, _L, _P, _P, _I, _L, _P, _Z, _P, _P]
+_SIGS["aeoq_moe_fp8_block_workspace_size"] = [_L, _L, _L, _L, _L]
+_SIGS["aeoq_moe_fp8_block_forward"] = [_P, _L, _P, _I, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P, _P, _Z, _P, _P]
+_RESTYPE = {"aeoq_fp8_block_linear_workspace_size": C.c_size_t,
+            "aeoq_moe_fp8_block_workspace_size": C.c_size_t,
+            "aeoq_moe_nvfp4_decode_tc_workspace_size": C.c_size_t,
             "aeoq_ep_nccl_unique_id_bytes": C.c_size_t, "aeoq_ep_dispatch_workspace_size": C.c_size_t,
             "aeoq_ep_experts_nvfp4_workspace_size": C.c_size_t, "aeoq_ep_combine_workspace_size": C.c_size_t,
             "aeoq_moe_nvfp4_decode_stream_workspace_size": C.c_size_t,
@@ -201,6 +211,15 @@ def err_word(device: torch.device) -> torch.Tensor:
         t = torch.zeros(1, dtype=torch.int32, device=device)
         _ERR_WORDS[key] = t
     return t
+
+
+def err_ptr(device: torch.device):
+    """Address of the error word, or None (kernels then record nothing) when
+    it does not exist yet and a graph is being captured: made there, it
+    would live in that graph's memory."""
+    if device.index not in _ERR_WORDS and torch.cuda.is_current_stream_capturing():
+        return None
+    return err_word(device).data_ptr()
 
 
 # Weight scale atoms are derived once per weight tensor and cached here,

@@ -364,3 +364,68 @@ def fp8_experts_grouped(hidden, top_k_index, top_k_weights, gu, gu_sb, dw, dw_sb
     A.check(lib.aeoq_moe_combine(c.data_ptr(), r.pair_row.data_ptr(), r.ids.data_ptr(), A.dtype_code(r.ids.dtype),
                                  T, k, H, 0, out.data_ptr(), st))                          # (:142-145)
     return out
+
+
+# ---------------------------------------------------------------- block-scaled FP8 experts
+_ACTIVATIONS = {"gelu_pytorch_tanh": A.ACT_GELU_TANH, "gelu_tanh": A.ACT_GELU_TANH, "silu": A.ACT_SILU}
+
+
+def fp8_block_experts(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale, activation="gelu_pytorch_tanh"):
+    """Routed experts with e4m3 weights that carry one f32 scale per 128 x 128
+    block: ``out[t] = sum_j w[t, j] * down(act(gate x) * up x)`` over the
+    experts ``top_k_index[t]``, any number of tokens, no host sync.
+
+    ``hidden`` (T, H) bfloat16, quantized per 128 values of a row, as the
+    experts' intermediate rows are; ``gu`` (E, 2I, H) with ``gu_scale`` (E,
+    ceil(2I/128), ceil(H/128)), ``dw`` (E, H, I) with ``dw_scale`` (E,
+    ceil(H/128), ceil(I/128)); an id outside [0, E) adds nothing. Sums are
+    f32; the output is bfloat16. H must be a multiple of 16, I of 64."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if hidden.ndim != 2 or hidden.dtype != torch.bfloat16:
+        raise ValueError(f"hidden_states must be bfloat16 (tokens, hidden), got {hidden.dtype} {tuple(hidden.shape)}")
+    if gu.ndim != 3 or dw.ndim != 3:
+        raise ValueError("expert weights must be 3D (experts, out, in)")
+    E, two_i, H = gu.shape
+    I = two_i // 2
+    T = hidden.shape[0]
+    blocks = lambda n: -(-n // 128)  # noqa: E731
+    if hidden.shape[1] != H or tuple(dw.shape) != (E, H, I) or two_i % 2:
+        raise ValueError(f"hidden {tuple(hidden.shape)}, gate_up {tuple(gu.shape)} and down {tuple(dw.shape)} "
+                         "do not fit together")
+    for name, t, s, want in (("gate_up", gu, gu_scale, (E, blocks(two_i), blocks(H))),
+                             ("down", dw, dw_scale, (E, blocks(H), blocks(I)))):
+        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise ValueError(f"{name} must be float8_e4m3fn, got {t.dtype}")
+        if tuple(s.shape) != want or s.dtype != torch.float32:
+            raise ValueError(f"{name} scales must be float32 of shape {want}, got {s.dtype} {tuple(s.shape)}")
+        if not t.is_contiguous() or not s.is_contiguous():
+            raise ValueError(f"{name} weights and scales must be contiguous")
+    if top_k_index.ndim != 2 or top_k_index.shape[0] != T or top_k_index.shape != top_k_weights.shape:
+        raise ValueError(f"top_k_index {tuple(top_k_index.shape)} and top_k_weights {tuple(top_k_weights.shape)} "
+                         f"must both be ({T}, k)")
+    if top_k_index.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"top_k_index must be int32 or int64, got {top_k_index.dtype}")
+    if not top_k_weights.dtype.is_floating_point:
+        raise ValueError(f"top_k_weights must be floating point, got {top_k_weights.dtype}")
+    A.require_cuda(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale)
+    dev = hidden.device
+    for t in (top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale):
+        if t.device != dev:
+            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
+    lib = A.load()
+    k = top_k_index.shape[1]
+    with A.on_device(dev):
+        hidden = hidden.contiguous()
+        if hidden.data_ptr() % 16:
+            hidden = hidden.clone()
+        ids = top_k_index.contiguous()
+        w = top_k_weights.detach().to(torch.float32).contiguous()
+        out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+        n = lib.aeoq_moe_fp8_block_workspace_size(T, k, E, H, I)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        A.check(lib.aeoq_moe_fp8_block_forward(
+            hidden.data_ptr(), T, ids.data_ptr(), A.dtype_code(ids.dtype), w.data_ptr(), k, gu.data_ptr(),
+            gu_scale.data_ptr(), dw.data_ptr(), dw_scale.data_ptr(), E, H, I, _ACTIVATIONS[activation],
+            out.data_ptr(), ws.data_ptr(), n, A.err_ptr(dev), A.stream_ptr(dev)))
+    return out

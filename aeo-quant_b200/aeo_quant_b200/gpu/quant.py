@@ -113,6 +113,87 @@ def dequantize_2d_from_fp8(weight_fp8: torch.Tensor, scale_bf16: torch.Tensor) -
     return weight_fp8.to(torch.bfloat16) * scale_bf16
 
 
+FP8_BLOCK = 128
+
+
+def quantize_fp8_activation_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """FP8 values with one scale per 128 values of a row (the activation side
+    of ``gpu.fp8_block_matmul``): ``(x_fp8 (..., K) float8_e4m3fn,
+    x_scale (..., ceil(K/128)) float32)``.
+
+    Per block, with ``a = max(max|x|, 1e-30)``: ``scale = f32(a / 448)`` and
+    ``q = e4m3(f32(x * f32(448 / a)))``, rounded to nearest even. The last
+    block of a row may be short. A block that holds an infinity or a NaN has
+    a NaN scale. Not in the reference, whose FP8 scales are per row."""
+    if x.ndim < 1:
+        raise ValueError("quantize_fp8_activation_blocks expects at least one dimension")
+    dt = A.dtype_code(x.dtype)
+    if dt not in (A.BF16, A.F16, A.F32):
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    A.require_cuda(x)
+    K = x.shape[-1]
+    with A.on_device(x.device):
+        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        s = torch.empty(*x.shape[:-1], -(-K // FP8_BLOCK), dtype=torch.float32, device=x.device)
+        if x.numel() == 0:
+            return q, s
+        x2 = _rows_view(x)
+        rows = x2.shape[0]
+        if rows > 1 and x2.stride(0) < K:
+            x2 = x2.contiguous()                # broadcast or overlapping rows
+        A.check(A.load().aeoq_fp8_block_quantize_rows(x2.data_ptr(), dt, rows, K, x2.stride(0) if rows > 1 else K,
+                                                      q.data_ptr(), K, s.data_ptr(), A.stream_ptr(x.device)))
+    return q, s
+
+
+def quantize_3d_to_fp8_block(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """FP8 weights with one scale per 128 x 128 block: ``(weight_fp8
+    (E, out, in) float8_e4m3fn, scale (E, ceil(out/128), ceil(in/128))
+    float32)``, by the formulas of :func:`quantize_fp8_activation_blocks`."""
+    if weight.ndim != 3:
+        raise ValueError(
+            f"quantize_3d_to_fp8_block expects a 3D tensor (num_experts, out_dim, in_dim); "
+            f"got shape {tuple(weight.shape)}"
+        )
+    dt = A.dtype_code(weight.dtype)
+    if dt not in (A.BF16, A.F16, A.F32):
+        raise ValueError(f"unsupported dtype {weight.dtype}")
+    A.require_cuda(weight)
+    E, N, K = weight.shape
+    with A.on_device(weight.device):
+        w = weight.contiguous()
+        q = torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device=w.device)
+        s = torch.empty(E, -(-N // FP8_BLOCK), -(-K // FP8_BLOCK), dtype=torch.float32, device=w.device)
+        A.check(A.load().aeoq_fp8_block_quantize_weights(w.data_ptr(), dt, E, N, K, q.data_ptr(), s.data_ptr(),
+                                                         A.stream_ptr(w.device)))
+    return q, s
+
+
+def quantize_2d_to_fp8_block(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`quantize_3d_to_fp8_block` of one matrix."""
+    if weight.ndim != 2:
+        raise ValueError(
+            f"quantize_2d_to_fp8_block expects a 2D tensor (out_dim, in_dim); "
+            f"got shape {tuple(weight.shape)}"
+        )
+    q, s = quantize_3d_to_fp8_block(weight.unsqueeze(0))
+    return q.squeeze(0), s.squeeze(0)
+
+
+def dequantize_fp8_activation_blocks(x_fp8: torch.Tensor, x_scale: torch.Tensor) -> torch.Tensor:
+    """Inverse of :func:`quantize_fp8_activation_blocks` in float32, for
+    testing/validation only."""
+    return x_fp8.float() * x_scale.repeat_interleave(FP8_BLOCK, -1)[..., : x_fp8.shape[-1]]
+
+
+def dequantize_from_fp8_block(weight_fp8: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """Inverse of :func:`quantize_2d_to_fp8_block` and
+    :func:`quantize_3d_to_fp8_block` in float32, for testing/validation only."""
+    N, K = weight_fp8.shape[-2:]
+    return (weight_fp8.float()
+            * scale.repeat_interleave(FP8_BLOCK, -2)[..., :N, :].repeat_interleave(FP8_BLOCK, -1)[..., :K])
+
+
 def quantize_3d_to_nvfp4(
     weight_bf16: torch.Tensor, block_size: int = NVFP4_BLOCK_SIZE
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -1,0 +1,197 @@
+// Block-scaled FP8 quantizers (formulas in fp8_block.cuh).
+//
+// Rows: a half-warp holds one block of 128 values, 8 per lane, in registers:
+// one 16-byte load (two for f32), four shuffles for the maximum, one 8-byte
+// store of codes. Weights: one CTA holds a 128 x 128 block in registers.
+// Every input value is read once, so both are bound by HBM.
+#include <algorithm>
+
+#include "fp8_block.cuh"
+
+namespace aeoq {
+
+constexpr int kFbRowWarps = 8;
+
+// One warp per row and run of `chunk` blocks. VEC: rows, their pieces of 8
+// and the code rows are aligned for wide accesses and K % 8 == 0.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(32 * kFbRowWarps) fb_rows_kernel(
+    const typename In<DT>::T* __restrict__ x, int64_t rows, int64_t K, int64_t ld, const int* __restrict__ idx,
+    const int* __restrict__ n_rows, int chunk, uint8_t* __restrict__ q, int64_t q_ld, float* __restrict__ scale) {
+  const int64_t r = blockIdx.x * (int64_t)kFbRowWarps + (threadIdx.x >> 5);
+  if (r >= rows || (n_rows && r >= *n_rows)) return;
+  const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
+  const typename In<DT>::T* xr = x + (idx ? (int64_t)idx[r] : r) * ld;
+  uint8_t* qr = q + r * q_ld;
+  const int nb = (int)fb_blocks(K);
+  float* sr = scale + r * nb;
+  const int b_end = min(nb, ((int)blockIdx.y + 1) * chunk);
+  constexpr int U = 4;   // blocks in flight per half-warp
+  for (int b0 = (int)blockIdx.y * chunk; b0 < b_end; b0 += 2 * U) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = b0 + 2 * u + half;
+      const int64_t k0 = (int64_t)b * kFbBlock + 8 * sub;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+      if (b < b_end && k0 < K) {
+        if (VEC) {
+          fb_load8<DT>(xr + k0, v[u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k0 + i < K) v[u][i] = In<DT>::load(xr + k0 + i);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = b0 + 2 * u + half;
+      const int64_t k0 = (int64_t)b * kFbBlock + 8 * sub;
+      uint32_t key = fb_key8(v[u]);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
+      const float2 s = fb_scales(fb_key_value(key));
+      if (b >= b_end) continue;
+      if (sub == 0) sr[b] = s.y;
+      const uint2 c = fb_codes8(v[u], s.x);
+      if (VEC) {
+        if (k0 < K) *reinterpret_cast<uint2*>(qr + k0) = c;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k0 + i < K) qr[k0 + i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+      }
+    }
+  }
+}
+
+// One 128 x 128 block per CTA: thread t holds columns 8 (t % 16) .. + 7 of
+// rows t / 16 + 16 i.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) fb_weights_kernel(const typename In<DT>::T* __restrict__ x, int64_t N,
+                                                         int64_t K, uint8_t* __restrict__ q,
+                                                         float* __restrict__ scale) {
+  __shared__ uint32_t part[8];
+  const int64_t e = blockIdx.z, nb = blockIdx.y, kb = blockIdx.x;
+  const int64_t k0 = kb * kFbBlock + 8 * (threadIdx.x & 15);
+  const int64_t n0 = nb * kFbBlock + (threadIdx.x >> 4);
+  const typename In<DT>::T* xe = x + e * N * K;
+  float v[8][8];
+  uint32_t key = 0;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const int64_t n = n0 + 16 * r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
+    if (n < N && k0 < K) {
+      if (VEC) {
+        fb_load8<DT>(xe + n * K + k0, v[r]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k0 + i < K) v[r][i] = In<DT>::load(xe + n * K + k0 + i);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) key = max(key, fb_key8(v[r]));
+  key = __reduce_max_sync(0xFFFFFFFFu, key);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = key;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) key = max(key, part[i]);
+  const float2 s = fb_scales(fb_key_value(key));
+  if (threadIdx.x == 0) scale[(e * gridDim.y + nb) * gridDim.x + kb] = s.y;
+  uint8_t* qe = q + e * N * K;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const int64_t n = n0 + 16 * r;
+    if (n >= N || k0 >= K) continue;
+    const uint2 c = fb_codes8(v[r], s.x);
+    if (VEC) {
+      *reinterpret_cast<uint2*>(qe + n * K + k0) = c;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k0 + i < K) qe[n * K + k0 + i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+    }
+  }
+}
+
+template <int DT>
+static int launch_rows(const void* x, int64_t rows, int64_t K, int64_t ld, const int* idx, const int* n_rows,
+                       uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st) {
+  using T = typename In<DT>::T;
+  const bool vec = K % 8 == 0 && (uintptr_t)x % 16 == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0 &&
+                   (uintptr_t)q % 8 == 0 && q_ld % 8 == 0;
+  const int64_t nb = fb_blocks(K);
+  // Few rows: split a row over warps until the GPU has some, in runs of
+  // whole iterations (8 blocks), then of 2 blocks.
+  const int64_t groups = (rows + kFbRowWarps - 1) / kFbRowWarps;
+  int64_t chunk = nb;
+  if (groups * 2 <= device_sm_count()) chunk = groups * ((nb + 7) / 8) >= device_sm_count() ? 8 : 2;
+  dim3 grid((unsigned)groups, (unsigned)((nb + chunk - 1) / chunk));
+  if (vec)
+    fb_rows_kernel<DT, true><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld, idx,
+                                                                n_rows, (int)chunk, q, q_ld, scale);
+  else
+    fb_rows_kernel<DT, false><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld, idx,
+                                                                 n_rows, (int)chunk, q, q_ld, scale);
+  return check_launch("fb_rows_kernel");
+}
+
+int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, const int* idx,
+                     const int* n_rows, uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st) {
+  switch (dtype) {
+    case AEOQ_BF16: return launch_rows<AEOQ_BF16>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
+    case AEOQ_F16: return launch_rows<AEOQ_F16>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
+    case AEOQ_F32: return launch_rows<AEOQ_F32>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
+  }
+  return set_error(AEOQ_ERR_INVALID, "fp8_block_quantize_rows: unsupported dtype %d", dtype);
+}
+
+template <int DT>
+static int launch_weights(const void* x, int64_t E, int64_t N, int64_t K, uint8_t* q, float* scale, cudaStream_t st) {
+  using T = typename In<DT>::T;
+  const bool vec = K % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)q % 8 == 0;
+  dim3 grid((unsigned)fb_blocks(K), (unsigned)fb_blocks(N), (unsigned)E);
+  if (vec)
+    fb_weights_kernel<DT, true><<<grid, 256, 0, st>>>(reinterpret_cast<const T*>(x), N, K, q, scale);
+  else
+    fb_weights_kernel<DT, false><<<grid, 256, 0, st>>>(reinterpret_cast<const T*>(x), N, K, q, scale);
+  return check_launch("fb_weights_kernel");
+}
+
+}  // namespace aeoq
+
+using namespace aeoq;
+
+extern "C" int aeoq_fp8_block_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, uint8_t* q,
+                                            int64_t q_ld, float* scale, void* stream) {
+  AEOQ_REQUIRE(dtype == AEOQ_BF16 || dtype == AEOQ_F16 || dtype == AEOQ_F32, AEOQ_ERR_INVALID,
+               "fp8_block_quantize_rows: unsupported dtype %d", dtype);
+  AEOQ_REQUIRE(rows >= 0 && K >= 0 && ld >= K && q_ld >= K, AEOQ_ERR_INVALID, "fp8_block_quantize_rows: bad shape");
+  AEOQ_REQUIRE(K <= (1LL << 24) && rows <= (1LL << 33), AEOQ_ERR_INVALID,
+               "fp8_block_quantize_rows: K at most 2^24, rows at most 2^33");
+  if (rows == 0 || K == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(x && q && scale, AEOQ_ERR_INVALID, "fp8_block_quantize_rows: null pointer");
+  return fb_quantize_rows(x, dtype, rows, K, ld, nullptr, nullptr, q, q_ld, scale, (cudaStream_t)stream);
+}
+
+extern "C" int aeoq_fp8_block_quantize_weights(const void* x, int dtype, int64_t num_experts, int64_t N, int64_t K,
+                                               uint8_t* q, float* scale, void* stream) {
+  AEOQ_REQUIRE(num_experts >= 0 && N >= 0 && K >= 0, AEOQ_ERR_INVALID, "fp8_block_quantize_weights: bad shape");
+  AEOQ_REQUIRE(num_experts <= 65535 && fb_blocks(N) <= 65535 && K <= (1LL << 31), AEOQ_ERR_INVALID,
+               "fp8_block_quantize_weights: at most 65535 matrices of 65535 x 128 rows");
+  if (num_experts == 0 || N == 0 || K == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(x && q && scale, AEOQ_ERR_INVALID, "fp8_block_quantize_weights: null pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case AEOQ_BF16: return launch_weights<AEOQ_BF16>(x, num_experts, N, K, q, scale, st);
+    case AEOQ_F16: return launch_weights<AEOQ_F16>(x, num_experts, N, K, q, scale, st);
+    case AEOQ_F32: return launch_weights<AEOQ_F32>(x, num_experts, N, K, q, scale, st);
+  }
+  return set_error(AEOQ_ERR_INVALID, "fp8_block_quantize_weights: unsupported dtype %d", dtype);
+}

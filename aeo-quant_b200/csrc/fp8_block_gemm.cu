@@ -1,0 +1,673 @@
+// Block-scaled FP8 GEMMs on the 5th-generation tensor cores (tcgen05), and
+// the routed experts' forward built on them.
+//
+//   y[m][n] = sum_b sa[m][b] * sw[n / 128][b] * ( sum_{k in block b} a[m][k] w[n][k] )
+//
+// a: e4m3 rows (tokens), w: e4m3 rows (output features), one f32 scale per
+// 128 values of a row of a and per 128 x 128 block of w.
+//
+// The tensor core sums one block b (four MMAs of K = 32) into TMEM; the
+// epilogue warps read that partial sum, multiply it by its two scales and
+// add it to f32 sums in registers. The blocks alternate between two TMEM
+// buffers, so the scaling of block b runs under the MMAs of block b + 1.
+// Tokens are the MMA's 128 rows: a TMEM lane is a token and a thread owns
+// one token, so its scale sa is one value per block and sw is the same for a
+// whole run of columns: the scaling is one packed f32 fma per two sums.
+//
+//   warp 0      TMA: per 128-wide K step one tile of a and one of w
+//               (128-byte swizzle)
+//   warp 1      TMEM owner and MMA issuer
+//   warps 4-11  scaling and epilogue: two warps per TMEM lane quadrant, each
+//               with half of the columns (128 f32 sums per thread: the two
+//               other warps only exist so that setmaxnreg can give their
+//               registers to these)
+//
+// One CTA per SM walks the tiles, output features fastest (they share the
+// tile of a in L2).
+//
+// Epilogues: store (bf16 or f32, optional bias); GLU: the tile holds 128
+// gate columns and the 128 up columns they pair with, h = act(g) * u is
+// quantized per 128 in the epilogue and written as the next GEMM's operand.
+#include <algorithm>
+
+#include "fp8_block.cuh"
+#include "sm100.cuh"
+
+namespace aeoq {
+
+int make_tmap_bytes(CUtensorMap* m, const void* ptr, int64_t rows, int64_t row_bytes, int64_t ld, int box_bytes,
+                    int box_rows, bool swizzle128);
+
+constexpr int kFbEpiWarps = 8;
+constexpr int kFbThreads = 128 + 32 * kFbEpiWarps;
+// Registers per thread after the split: 128 x 56 + 256 x 224 = 64512, what
+// the block is launched with (384 x 168).
+constexpr int kFbRegsLow = 56, kFbRegsHigh = 224;
+constexpr int kFbMaxStages = 8;
+constexpr int kFbMaxExperts = 1024;
+
+enum FbEpilogue : int { kFbStore = 0, kFbGlu = 1 };
+enum FbActivation : int { kFbGeluTanh = 0, kFbSilu = 1 };
+
+struct FbParams {
+  int64_t M;              // rows of a (dense), or the most there can be (grouped)
+  int64_t N;              // rows of w per expert
+  int K, KB;              // K and its blocks
+  int64_t NB;             // scale rows per expert, ceil(N / 128)
+  int E;
+  const float* sa;        // (rows of a, KB)
+  const float* sw;        // (E, NB, KB)
+  const int* grp_off;     // grouped: rows [grp_off[e], grp_off[e + 1]) are expert e's; null: dense
+  const int* tile_off;    // grouped: tiles of 128 rows before expert e's, E + 1 values
+  int64_t tiles_m;        // dense
+  int tiles_n;
+  void* out; int out_dt; int64_t ldc;   // store: row stride in elements
+  const __nv_bfloat16* bias;            // store: N values or null
+  int64_t I;              // GLU: gate rows are w rows [0, I), up rows [I, 2 I)
+  int act;
+  uint8_t* hq; int64_t hq_ld;           // GLU: quantized h rows
+  float* hs; int64_t hs_ld;             // GLU: their scales, (rows, ceil(I / 128))
+  int* err;
+};
+
+template <int BN>
+struct FbLayout {
+  static constexpr uint32_t kA = 128 * 128, kB = BN * 128, kStage = kA + kB;
+  struct Ctl {
+    uint64_t full[kFbMaxStages], empty[kFbMaxStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    float amax[2][128];                // GLU: the two column halves' maxima per row
+    int tile_off[kFbMaxExperts + 1];
+  };
+  static constexpr int kStages = std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl)) / (int)kStage);
+  static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + sizeof(Ctl);
+  static constexpr uint32_t kTmemCols = 2 * BN;
+};
+
+struct FbTile {
+  int64_t expert, row0, n0;   // first row of a, first column (GLU: first gate column)
+  int rows;                   // valid rows
+};
+
+template <int BN, int EPI>
+__device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off, int64_t t) {
+  FbTile r;
+  const int64_t mt = t / p.tiles_n;
+  r.n0 = (t - mt * p.tiles_n) * (EPI == kFbGlu ? BN / 2 : BN);
+  if (!p.grp_off) {
+    r.expert = 0;
+    r.row0 = mt * 128;
+    r.rows = (int)min((int64_t)128, p.M - r.row0);
+    return r;
+  }
+  int lo = 0, hi = p.E;       // the expert e with tile_off[e] <= mt < tile_off[e + 1]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile_off[mid] <= mt) lo = mid; else hi = mid;
+  }
+  r.expert = lo;
+  const int64_t in = (mt - tile_off[lo]) * 128;
+  const int64_t g0 = __ldg(p.grp_off + lo), g1 = __ldg(p.grp_off + lo + 1);
+  r.row0 = g0 + in;
+  r.rows = (int)min((int64_t)128, g1 - r.row0);
+  return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
+// gelu(x, tanh form) = x * sigmoid(2 z), z = sqrt(2/pi) (x + 0.044715 x^3),
+// since 1 + tanh(z) = 2 sigmoid(2 z); silu(x) = x * sigmoid(x). Written so,
+// neither cancels for negative x. __expf's relative error grows with its
+// argument (about 2^-22 + |arg| 2^-24); where |arg| is large the result is 0
+// or x to within f32.
+__device__ __forceinline__ float fb_act(int act, float x) {
+  const float a = act == kFbSilu ? x : 1.5957691216057308f * (x + 0.044715f * (x * x * x));
+  return __fdividef(x, 1.0f + __expf(-a));
+}
+
+template <int BN, int EPI>
+__global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                                      const __grid_constant__ CUtensorMap tmW,
+                                                                      const FbParams p) {
+  using L = FbLayout<BN>;
+  extern __shared__ __align__(1024) uint8_t dsmem[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
+  auto* sh = reinterpret_cast<typename L::Ctl*>(base + L::kStages * L::kStage);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      sm100::mbar_init(&sh->full[s], 1);
+      sm100::mbar_init(&sh->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      sm100::mbar_init(&sh->acc_full[b], 1);
+      sm100::mbar_init(&sh->acc_empty[b], kFbEpiWarps);
+    }
+    sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tmA);
+    sm100::prefetch_tmap(&tmW);
+  }
+  if (p.grp_off)
+    for (int e = tid; e <= p.E; e += kFbThreads) sh->tile_off[e] = p.tile_off[e];
+  if (warp == 1) sm100::tmem_alloc(&sh->tmem_base, L::kTmemCols);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const int64_t total = (p.grp_off ? (int64_t)sh->tile_off[p.E] : p.tiles_m) * p.tiles_n;
+  const int KB = p.KB;
+
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFbRegsLow));
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const bool leader = sm100::elect_one();
+    uint32_t g = 0;      // K steps so far
+    bool alive = true;
+    for (int64_t t = blockIdx.x; t < total && alive; t += gridDim.x) {
+      const FbTile ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
+      const int64_t w0 = ti.expert * p.N + ti.n0;
+      for (int kb = 0; kb < KB; ++kb, ++g) {
+        const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
+        if (!sm100::mbar_wait(&sh->empty[s], ph ^ 1, p.err, 71)) { alive = false; break; }
+        if (leader) {
+          uint8_t* st = base + s * L::kStage;
+          sm100::mbar_arrive_expect_tx(&sh->full[s], L::kStage);
+          sm100::tma_load_2d(st, &tmA, kb * 128, (int32_t)ti.row0, &sh->full[s]);
+          sm100::tma_load_2d(st + L::kA, &tmW, kb * 128, (int32_t)w0, &sh->full[s]);
+          if constexpr (EPI == kFbGlu)
+            sm100::tma_load_2d(st + L::kA + L::kB / 2, &tmW, kb * 128, (int32_t)(w0 + p.I), &sh->full[s]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    const bool leader = sm100::elect_one();
+    constexpr uint32_t idesc = sm100::idesc_f8(BN);
+    uint32_t g = 0;
+    bool alive = true;
+    for (int64_t t = blockIdx.x; t < total && alive; t += gridDim.x) {
+      for (int kb = 0; kb < KB; ++kb, ++g) {
+        const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
+        const uint32_t b = g & 1, bph = (g >> 1) & 1;
+        if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72) ||
+            !sm100::mbar_wait(&sh->full[s], ph, p.err, 73)) { alive = false; break; }
+        sm100::tc_fence_after();
+        if (leader) {
+          const uint32_t sa = sm100::smem_u32(base + s * L::kStage), sb = sa + L::kA;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sm100::tc_mma_f8(tmem + b * BN, sm100::sdesc_k_sw128(sa + 32 * j), sm100::sdesc_k_sw128(sb + 32 * j),
+                             idesc, j ? 1u : 0u);
+          sm100::tc_commit(&sh->empty[s]);
+          sm100::tc_commit(&sh->acc_full[b]);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFbRegsHigh));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const int row = 32 * q + lane;
+    constexpr int kCols = BN / 2;          // columns of this thread
+    constexpr int kChunks = kCols / 32;
+    // first TMEM column of chunk c, and which of the two weight scales it has
+    auto col_of = [&](int c) {
+      if constexpr (EPI == kFbGlu)
+        return c < kChunks / 2 ? half * (BN / 4) + 32 * c : BN / 2 + half * (BN / 4) + 32 * (c - kChunks / 2);
+      else
+        return half * kCols + 32 * c;
+    };
+    uint32_t g = 0;
+    // A warp whose wait ran out goes through its remaining tiles without
+    // waiting or storing: the other warps count on it at the barriers below.
+    bool alive = true;
+    for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+      const FbTile ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
+      const bool live = row < ti.rows;
+      const float* sa = p.sa + (ti.row0 + (live ? row : 0)) * KB;
+      const float *sw0, *sw1;
+      {
+        const float* se = p.sw + ti.expert * p.NB * KB;
+        // a run of columns that lies past the last row of w reads the last
+        // scale; its sums are not used
+        const int64_t c0 = min(ti.n0 + col_of(0), p.N - 1);
+        const int64_t c1 = EPI == kFbGlu ? min(p.I + ti.n0 + half * (BN / 4), p.N - 1) : c0;
+        sw0 = se + (c0 / kFbBlock) * KB;
+        sw1 = se + (c1 / kFbBlock) * KB;
+      }
+      uint64_t acc[kCols / 2];
+#pragma unroll
+      for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
+      float a = __ldg(sa), w0 = __ldg(sw0), w1 = __ldg(sw1);
+      for (int kb = 0; kb < KB; ++kb, ++g) {
+        const uint32_t b = g & 1, bph = (g >> 1) & 1;
+        const float c0 = a * w0, c1 = a * w1;
+        const uint64_t cc0 = pack2(c0, c0), cc1 = pack2(c1, c1);
+        if (kb + 1 < KB) {
+          a = __ldg(sa + kb + 1);
+          w0 = __ldg(sw0 + kb + 1);
+          w1 = __ldg(sw1 + kb + 1);
+        }
+        if (!alive || !sm100::mbar_wait(&sh->acc_full[b], bph, p.err, 74)) {
+          alive = false;
+          break;
+        }
+        sm100::tc_fence_after();
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t r[32];
+          sm100::tmem_ld32_nowait(tq + col_of(c), r);
+          sm100::tmem_ld_wait();
+          if (c == kChunks - 1) {
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&sh->acc_empty[b]);
+          }
+          const uint64_t cc = (EPI == kFbGlu && c >= kChunks / 2) ? cc1 : cc0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            acc[16 * c + i] =
+                fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), cc, acc[16 * c + i]);
+        }
+      }
+      if constexpr (EPI == kFbStore) {
+        if (!live || !alive) continue;
+        const int64_t n0 = ti.n0 + half * kCols;
+        const int64_t o = (ti.row0 + row) * p.ldc + n0;
+        if (p.bias) {
+#pragma unroll
+          for (int i = 0; i < kCols / 2; ++i) {
+            const float2 v = unpack2(acc[i]);
+            const float b0 = n0 + 2 * i < p.N ? __bfloat162float(p.bias[n0 + 2 * i]) : 0.0f;
+            const float b1 = n0 + 2 * i + 1 < p.N ? __bfloat162float(p.bias[n0 + 2 * i + 1]) : 0.0f;
+            acc[i] = pack2(v.x + b0, v.y + b1);
+          }
+        }
+        const int64_t left = p.N - n0;     // columns of this thread that exist
+        if (p.out_dt == AEOQ_BF16) {
+          __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + o;
+          const bool wide = p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+#pragma unroll
+          for (int i = 0; i < kCols / 8; ++i) {
+            __align__(16) __nv_bfloat162 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack2(acc[4 * i + j]);
+              v[j] = __floats2bfloat162_rn(f.x, f.y);
+            }
+            if (wide && 8 * i + 8 <= left) {
+              *reinterpret_cast<uint4*>(d + 8 * i) = *reinterpret_cast<const uint4*>(v);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (8 * i + j < left) d[8 * i + j] = j & 1 ? v[j / 2].y : v[j / 2].x;
+            }
+          }
+        } else {
+          float* d = reinterpret_cast<float*>(p.out) + o;
+          const bool wide = p.ldc % 4 == 0 && (uintptr_t)p.out % 16 == 0;
+#pragma unroll
+          for (int i = 0; i < kCols / 4; ++i) {
+            const float2 u = unpack2(acc[2 * i]), v = unpack2(acc[2 * i + 1]);
+            if (wide && 4 * i + 4 <= left) {
+              *reinterpret_cast<float4*>(d + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
+            } else {
+              if (4 * i < left) d[4 * i] = u.x;
+              if (4 * i + 1 < left) d[4 * i + 1] = u.y;
+              if (4 * i + 2 < left) d[4 * i + 2] = v.x;
+              if (4 * i + 3 < left) d[4 * i + 3] = v.y;
+            }
+          }
+        }
+      } else {
+        // h = act(gate) * up of this thread's BN / 4 columns; columns past I
+        // (and rows past the tile's) count as zeros
+        constexpr int kH = BN / 4;
+        const int64_t n0 = ti.n0 + half * kH;
+        const int n_ok = (int)min((int64_t)kH, p.I - n0);
+        float h[kH];
+        uint32_t key = 0;
+#pragma unroll
+        for (int i = 0; i < kH / 2; ++i) {
+          const float2 gt = unpack2(acc[i]), up = unpack2(acc[kH / 2 + i]);
+          h[2 * i] = 2 * i < n_ok ? fb_act(p.act, gt.x) * up.x : 0.0f;
+          h[2 * i + 1] = 2 * i + 1 < n_ok ? fb_act(p.act, gt.y) * up.y : 0.0f;
+          key = max(key, __float_as_uint(h[2 * i]) & 0x7FFFFFFFu);
+          key = max(key, __float_as_uint(h[2 * i + 1]) & 0x7FFFFFFFu);
+        }
+        sh->amax[half][row] = __uint_as_float(key);
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kFbEpiWarps) : "memory");
+        key = max(key, __float_as_uint(sh->amax[half ^ 1][row]));
+        // the next tile's maxima are written after every read of these
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kFbEpiWarps) : "memory");
+        const float2 s = fb_scales(__uint_as_float(key));
+        if (live && alive) {
+          if (half == 0) p.hs[(ti.row0 + row) * p.hs_ld + ti.n0 / kFbBlock] = s.y;
+          uint8_t* d = p.hq + (ti.row0 + row) * p.hq_ld + n0;
+#pragma unroll
+          for (int i = 0; i < kH / 16; ++i) {
+            if (16 * i >= n_ok) break;
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float* v = h + 16 * i + 4 * j;
+              c[j] = fb_codes4(v[0] * s.x, v[1] * s.x, v[2] * s.x, v[3] * s.x);
+            }
+            *reinterpret_cast<uint4*>(d + 16 * i) = make_uint4(c[0], c[1], c[2], c[3]);
+          }
+        }
+      }
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+template <int BN, int EPI>
+static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, const FbParams& p, int64_t max_tiles,
+                       cudaStream_t st) {
+  using L = FbLayout<BN>;
+  CUtensorMap ta, tw;
+  int rc = make_tmap_bytes(&ta, a, a_rows, p.K, p.K, 128, 128, true);
+  if (rc) return rc;
+  rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, EPI == kFbGlu ? BN / 2 : BN, true);
+  if (rc) return rc;
+  rc = func_smem_attr((const void*)fp8_block_gemm_kernel<BN, EPI>, L::kBytes, -1, "fp8_block_gemm");
+  if (rc) return rc;
+  const int ctas = (int)std::min<int64_t>(device_sm_count(), max_tiles);
+  fp8_block_gemm_kernel<BN, EPI><<<ctas, kFbThreads, L::kBytes, st>>>(ta, tw, p);
+  return check_launch("fp8_block_gemm_kernel");
+}
+
+static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_t* w, const float* sw, int64_t N,
+                      int64_t K, const void* bias, void* out, int out_dt, int64_t ldc, int* err, cudaStream_t st) {
+  FbParams p{};
+  p.M = M;
+  p.N = N;
+  p.K = (int)K;
+  p.KB = (int)fb_blocks(K);
+  p.NB = fb_blocks(N);
+  p.E = 1;
+  p.sa = sa;
+  p.sw = sw;
+  p.tiles_m = (M + 127) / 128;
+  p.out = out;
+  p.out_dt = out_dt;
+  p.ldc = ldc;
+  p.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
+  p.err = err;
+  p.tiles_n = (int)((N + 127) / 128);
+  if (p.tiles_m * ((N + 255) / 256) < device_sm_count())
+    return launch_gemm<128, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
+  p.tiles_n = (int)((N + 255) / 256);
+  return launch_gemm<256, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
+}
+
+// ---------------------------------------------------------------- experts
+// Pairs (token, slot) sorted by expert: a counting sort in one CTA.
+//   grp_off[e]   first row of expert e        (E + 1 values)
+//   tile_off[e]  128-row tiles before expert e (E + 1 values)
+//   row_tok[r]   token of sorted row r;  pair_row[i]  row of pair i, or -1
+__global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_dt, int64_t n_pairs, int k, int E,
+                                                       int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
+  __shared__ int cnt[kFbMaxExperts], fill[kFbMaxExperts];
+  __shared__ int s_row[32], s_tile[32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  cnt[t] = 0;
+  __syncthreads();
+  for (int64_t i = t; i < n_pairs; i += 1024) {
+    const int64_t e = load_index(ids, ids_dt, i);
+    if (e >= 0 && e < E) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  const int c = cnt[t], d = (c + 127) / 128;      // experts past E count 0
+  int r = c, q = d;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int rr = __shfl_up_sync(0xFFFFFFFFu, r, o), qq = __shfl_up_sync(0xFFFFFFFFu, q, o);
+    if (lane >= o) { r += rr; q += qq; }
+  }
+  if (lane == 31) { s_row[warp] = r; s_tile[warp] = q; }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) { r += s_row[w]; q += s_tile[w]; }
+  fill[t] = r - c;
+  if (t < E) {
+    grp_off[t] = r - c;
+    tile_off[t] = q - d;
+    if (t == E - 1) { grp_off[E] = r; tile_off[E] = q; }
+  }
+  __syncthreads();
+  for (int64_t i = t; i < n_pairs; i += 1024) {
+    const int64_t e = load_index(ids, ids_dt, i);
+    int at = -1;
+    if (e >= 0 && e < E) {
+      at = atomicAdd(&fill[e], 1);
+      row_tok[at] = (int)(i / k);
+    }
+    pair_row[i] = at;
+  }
+}
+
+// out[t] = sum over slots j, in order, of weights[t][j] * y[pair_row[t][j]], in
+// f32, rounded once; a slot without an expert adds nothing.
+__global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __restrict__ y,
+                                                         const int* __restrict__ pair_row,
+                                                         const float* __restrict__ weights, int64_t T, int k,
+                                                         int64_t H, __nv_bfloat16* __restrict__ out) {
+  const int64_t per = H / 8, n = T * per;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t t = i / per, c = i - t * per;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < k; ++j) {
+      const int r = __ldg(pair_row + t * k + j);
+      if (r < 0) continue;
+      const float w = __ldg(weights + t * k + j);
+      float v[8];
+      fb_load8<AEOQ_BF16>(y + r * H + 8 * c, v);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) s[x] = fmaf(w, v[x], s[x]);
+    }
+    __align__(16) __nv_bfloat162 o[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[x] = __floats2bfloat162_rn(s[2 * x], s[2 * x + 1]);
+    *reinterpret_cast<uint4*>(out + t * H + 8 * c) = *reinterpret_cast<const uint4*>(o);
+  }
+}
+
+// Workspace of the grouped forward.
+struct FbExpertsWs {
+  size_t grp_off, tile_off, row_tok, pair_row, xq, xs, hq, hs, y, bytes;
+  FbExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+    size_t o = 0;
+    const int64_t P = T * k;
+    auto take = [&](int64_t n) {
+      const size_t at = o;
+      o += (size_t)((n + 255) / 256 * 256);
+      return at;
+    };
+    grp_off = take(4 * (E + 1));
+    tile_off = take(4 * (E + 1));
+    row_tok = take(4 * P);
+    pair_row = take(4 * P);
+    xq = take(P * H);
+    xs = take(4 * P * fb_blocks(H));
+    hq = take(P * I);
+    hs = take(4 * P * fb_blocks(I));
+    y = take(2 * P * H);
+    bytes = o;
+  }
+};
+
+}  // namespace aeoq
+
+using namespace aeoq;
+
+static int check_linear(const char* what, int64_t M, int64_t N, int64_t K, int out_dtype, int64_t ldc) {
+  AEOQ_REQUIRE(M >= 0 && N >= 0 && K >= 0, AEOQ_ERR_INVALID, "%s: negative shape", what);
+  AEOQ_REQUIRE(K > 0 && K % 16 == 0 && K <= (1LL << 24), AEOQ_ERR_INVALID,
+               "%s: K (%lld) must be a positive multiple of 16, at most 2^24", what, (long long)K);
+  AEOQ_REQUIRE(M <= 0x7FFFFFFF && N <= 0x7FFFFFFF, AEOQ_ERR_INVALID, "%s: M and N must fit 31 bits", what);
+  AEOQ_REQUIRE(out_dtype == AEOQ_BF16 || out_dtype == AEOQ_F32, AEOQ_ERR_INVALID, "%s: bad output dtype", what);
+  AEOQ_REQUIRE(ldc >= N, AEOQ_ERR_INVALID, "%s: output row stride %lld is below N", what, (long long)ldc);
+  return AEOQ_OK;
+}
+
+extern "C" int aeoq_fp8_block_gemm(const uint8_t* a, const float* sa, int64_t M, const uint8_t* w, const float* sw,
+                                   int64_t N, int64_t K, const void* bias, void* out, int out_dtype, int64_t ldc,
+                                   int* err_word, void* stream) {
+  int rc = check_linear("fp8_block_gemm", M, N, K, out_dtype, ldc);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(a && sa && w && sw && out, AEOQ_ERR_INVALID, "fp8_block_gemm: null pointer");
+  AEOQ_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0, AEOQ_ERR_INVALID,
+               "fp8_block_gemm: operands must be 16-byte aligned");
+  return gemm_dense(a, sa, M, w, sw, N, K, bias, out, out_dtype, ldc, err_word, (cudaStream_t)stream);
+}
+
+static size_t linear_scales_at(int64_t M, int64_t K) { return (size_t)((M * K + 255) / 256 * 256); }
+
+extern "C" size_t aeoq_fp8_block_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return linear_scales_at(M, K) + (size_t)M * fb_blocks(K) * 4;
+}
+
+extern "C" int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int64_t M, const uint8_t* w,
+                                     const float* sw, int64_t N, int64_t K, const void* bias, void* out,
+                                     int out_dtype, int64_t ldc, void* workspace, size_t workspace_bytes,
+                                     int* err_word, void* stream) {
+  int rc = check_linear("fp8_block_linear", M, N, K, out_dtype, ldc);
+  if (rc) return rc;
+  AEOQ_REQUIRE(dtype == AEOQ_BF16 || dtype == AEOQ_F16 || dtype == AEOQ_F32, AEOQ_ERR_INVALID,
+               "fp8_block_linear: unsupported input dtype %d", dtype);
+  AEOQ_REQUIRE(ldx >= K || M <= 1, AEOQ_ERR_INVALID, "fp8_block_linear: input row stride below K");
+  if (M == 0 || N == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(x && w && sw && out, AEOQ_ERR_INVALID, "fp8_block_linear: null pointer");
+  AEOQ_REQUIRE((uintptr_t)w % 16 == 0, AEOQ_ERR_INVALID, "fp8_block_linear: weights must be 16-byte aligned");
+  const size_t need = aeoq_fp8_block_linear_workspace_size(M, N, K);
+  AEOQ_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 256 == 0, AEOQ_ERR_WORKSPACE,
+               "fp8_block_linear: a 256-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  uint8_t* q = reinterpret_cast<uint8_t*>(workspace);
+  float* s = reinterpret_cast<float*>(q + linear_scales_at(M, K));
+  rc = fb_quantize_rows(x, dtype, M, K, ldx, nullptr, nullptr, q, K, s, st);
+  if (rc) return rc;
+  return gemm_dense(q, s, M, w, sw, N, K, bias, out, out_dtype, ldc, err_word, st);
+}
+
+extern "C" size_t aeoq_moe_fp8_block_workspace_size(int64_t T, int64_t top_k, int64_t num_experts, int64_t hidden,
+                                                    int64_t inter) {
+  if (T <= 0 || top_k <= 0 || num_experts <= 0 || hidden <= 0 || inter <= 0) return 0;
+  return FbExpertsWs(T, top_k, num_experts, hidden, inter).bytes;
+}
+
+extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const void* top_k_index, int idx_dtype,
+                                          const float* top_k_weights, int64_t top_k, const uint8_t* gate_up,
+                                          const float* gate_up_scale, const uint8_t* down, const float* down_scale,
+                                          int64_t num_experts, int64_t hidden_dim, int64_t inter_dim, int activation,
+                                          void* out, void* workspace, size_t workspace_bytes, int* err_word,
+                                          void* stream) {
+  const int64_t H = hidden_dim, I = inter_dim, E = num_experts, k = top_k;
+  AEOQ_REQUIRE(E >= 1 && E <= kFbMaxExperts, AEOQ_ERR_INVALID, "moe_fp8_block: 1 <= num_experts <= %d", kFbMaxExperts);
+  AEOQ_REQUIRE(k >= 1 && k <= 32, AEOQ_ERR_INVALID, "moe_fp8_block: 1 <= top_k <= 32");
+  AEOQ_REQUIRE(H >= 16 && H % 16 == 0 && H <= (1 << 24), AEOQ_ERR_INVALID,
+               "moe_fp8_block: hidden size (%lld) must be a multiple of 16", (long long)H);
+  AEOQ_REQUIRE(I >= 64 && I % 64 == 0 && I <= (1 << 24), AEOQ_ERR_INVALID,
+               "moe_fp8_block: intermediate size (%lld) must be a multiple of 64", (long long)I);
+  AEOQ_REQUIRE(E * 2 * I <= 0x7FFFFFFF && E * H <= 0x7FFFFFFF, AEOQ_ERR_INVALID,
+               "moe_fp8_block: the experts' weight rows must fit 31 bits");
+  AEOQ_REQUIRE(T >= 0 && T <= 0x7FFFFFFF / k, AEOQ_ERR_INVALID, "moe_fp8_block: bad token count");
+  AEOQ_REQUIRE(idx_dtype == AEOQ_I32 || idx_dtype == AEOQ_I64, AEOQ_ERR_INVALID, "moe_fp8_block: int32/int64 ids");
+  AEOQ_REQUIRE(activation == AEOQ_ACT_GELU_TANH || activation == AEOQ_ACT_SILU, AEOQ_ERR_INVALID,
+               "moe_fp8_block: bad activation %d", activation);
+  if (T == 0) return AEOQ_OK;
+  AEOQ_REQUIRE(hidden && top_k_index && top_k_weights && gate_up && gate_up_scale && down && down_scale && out,
+               AEOQ_ERR_INVALID, "moe_fp8_block: null pointer");
+  AEOQ_REQUIRE((uintptr_t)hidden % 16 == 0 && (uintptr_t)gate_up % 16 == 0 && (uintptr_t)down % 16 == 0 &&
+                   (uintptr_t)out % 16 == 0,
+               AEOQ_ERR_INVALID, "moe_fp8_block: hidden, weights and output must be 16-byte aligned");
+  const FbExpertsWs l(T, k, E, H, I);
+  AEOQ_REQUIRE(workspace && workspace_bytes >= l.bytes && (uintptr_t)workspace % 256 == 0, AEOQ_ERR_WORKSPACE,
+               "moe_fp8_block: a 256-byte aligned workspace of %zu bytes needed, %zu given", l.bytes, workspace_bytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  auto ints = [&](size_t o) { return reinterpret_cast<int*>(ws + o); };
+  auto floats = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
+  const int64_t P = T * k;
+  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, ints(l.grp_off), ints(l.tile_off),
+                                     ints(l.row_tok), ints(l.pair_row));
+  int rc = check_launch("fb_sort_kernel");
+  if (rc) return rc;
+  rc = fb_quantize_rows(hidden, AEOQ_BF16, P, H, H, ints(l.row_tok), ints(l.grp_off) + E, ws + l.xq, H,
+                        floats(l.xs), st);
+  if (rc) return rc;
+  const int64_t max_tiles = std::min<int64_t>(P, (P + 127) / 128 + E);
+  FbParams p{};
+  p.M = P;
+  p.N = 2 * I;
+  p.K = (int)H;
+  p.KB = (int)fb_blocks(H);
+  p.NB = fb_blocks(2 * I);
+  p.E = (int)E;
+  p.sa = floats(l.xs);
+  p.sw = gate_up_scale;
+  p.grp_off = ints(l.grp_off);
+  p.tile_off = ints(l.tile_off);
+  p.tiles_n = (int)fb_blocks(I);
+  p.I = I;
+  p.act = activation;
+  p.hq = ws + l.hq;
+  p.hq_ld = I;
+  p.hs = floats(l.hs);
+  p.hs_ld = fb_blocks(I);
+  p.err = err_word;
+  rc = launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
+  if (rc) return rc;
+  FbParams d{};
+  d.M = P;
+  d.N = H;
+  d.K = (int)I;
+  d.KB = (int)fb_blocks(I);
+  d.NB = fb_blocks(H);
+  d.E = (int)E;
+  d.sa = floats(l.hs);
+  d.sw = down_scale;
+  d.grp_off = ints(l.grp_off);
+  d.tile_off = ints(l.tile_off);
+  d.tiles_n = (int)((H + 255) / 256);
+  d.out = ws + l.y;
+  d.out_dt = AEOQ_BF16;
+  d.ldc = H;
+  d.err = err_word;
+  rc = launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
+  if (rc) return rc;
+  const int64_t pieces = T * (H / 8);
+  const unsigned blocks = (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)device_sm_count() * 16);
+  fb_combine_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(ws + l.y), ints(l.pair_row),
+                                            top_k_weights, T, (int)k, H, reinterpret_cast<__nv_bfloat16*>(out));
+  return check_launch("fb_combine_kernel");
+}

@@ -53,6 +53,10 @@ extern "C" {
 #define AEOQ_GROUP_MAX 0  /* the largest choice value of the group */
 #define AEOQ_GROUP_TOP2 1 /* the sum of its two largest */
 
+/* activation of a gated MLP */
+#define AEOQ_ACT_GELU_TANH 0
+#define AEOQ_ACT_SILU 1
+
 /* Library version (major*10000 + minor*100 + patch). */
 AEOQ_API int aeoq_version(void);
 
@@ -494,6 +498,71 @@ AEOQ_API int aeoq_moe_nvfp4_decode_fused_noalloc(const void* hidden, const void*
 AEOQ_API int aeoq_route_topk(const void* logits, int dtype, int64_t ld, int64_t T, int64_t num_experts, int64_t k,
                              int score, const float* bias, int64_t n_group, int64_t topk_group, int group_score,
                              int renormalize, float scale, float* weights, int64_t* ids, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Block-scaled FP8 quantizers: e4m3 values with one f32 scale per 128
+ * values. For a block with a = max(max|x|, 1e-30):
+ *   scale = f32(a / 448), inv = f32(448 / a), q = e4m3(f32(x * inv))
+ * (round to nearest even); a block that holds an infinity or a NaN gets a
+ * NaN scale and NaN codes. The last block of a row or column may be short.
+ * No counterpart in the reference, whose FP8 scales are per row.
+ *
+ * aeoq_fp8_block_quantize_rows: rows x K values of `dtype` (BF16/F16/F32),
+ * row stride ld; q rows of stride q_ld; scale (rows, ceil(K/128)) f32, one
+ * per 128 values of a row (activations).
+ * aeoq_fp8_block_quantize_weights: num_experts contiguous N x K matrices;
+ * scale (num_experts, ceil(N/128), ceil(K/128)) f32, one per 128 x 128 block.
+ * ------------------------------------------------------------------------ */
+AEOQ_API int aeoq_fp8_block_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, uint8_t* q,
+                                          int64_t q_ld, float* scale, void* stream);
+AEOQ_API int aeoq_fp8_block_quantize_weights(const void* x, int dtype, int64_t num_experts, int64_t N, int64_t K,
+                                             uint8_t* q, float* scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Block-scaled FP8 matrix product (tcgen05):
+ *   y[m][n] = sum_b sa[m][b] sw[n/128][b] sum_{k in block b} a[m][k] w[n][k] + bias[n]
+ * a (M, K) and w (N, K) e4m3, contiguous and 16-byte aligned; sa (M,
+ * ceil(K/128)) and sw (ceil(N/128), ceil(K/128)) f32; bias N bf16 values or
+ * null; out BF16 or F32 with a row stride of ldc elements. K % 16 == 0; M
+ * and N are free. err_word (a device int, or null) is set non-zero if a
+ * bounded wait runs out (never expected). No counterpart in the reference,
+ * whose FP8 linear has one scale per row (aeoq_fp8_gemm).
+ *
+ * aeoq_fp8_block_linear quantizes its input first
+ * (aeoq_fp8_block_quantize_rows; x BF16/F16/F32, row stride ldx) into the
+ * workspace, whose size aeoq_fp8_block_linear_workspace_size gives (256-byte
+ * aligned).
+ * ------------------------------------------------------------------------ */
+AEOQ_API int aeoq_fp8_block_gemm(const uint8_t* a, const float* sa, int64_t M, const uint8_t* w, const float* sw,
+                                 int64_t N, int64_t K, const void* bias, void* out, int out_dtype, int64_t ldc,
+                                 int* err_word, void* stream);
+AEOQ_API size_t aeoq_fp8_block_linear_workspace_size(int64_t M, int64_t N, int64_t K);
+AEOQ_API int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int64_t M, const uint8_t* w,
+                                   const float* sw, int64_t N, int64_t K, const void* bias, void* out,
+                                   int out_dtype, int64_t ldc, void* workspace, size_t workspace_bytes,
+                                   int* err_word, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Routed experts with block-scaled FP8 weights, any number of tokens, no
+ * host synchronisation:
+ *   x' = quantized hidden (per 128);  g, u = the two halves of gate_up x'
+ *   h = act(g) * u, quantized per 128;  y = down h
+ *   out[t] = sum_j top_k_weights[t][j] * y of expert top_k_index[t][j]
+ * hidden (T, H) bf16, contiguous; top_k_index (T, k) int32 or int64, an id
+ * outside [0, num_experts) adds nothing; top_k_weights (T, k) f32; gate_up
+ * (E, 2I, H) and down (E, H, I) e4m3; their scales (E, ceil(2I/128),
+ * ceil(H/128)) and (E, ceil(H/128), ceil(I/128)) f32; out (T, H) bf16.
+ * H % 16 == 0, I % 64 == 0, k <= 32, E <= 1024. Sums are f32, the experts'
+ * outputs are held in bf16 before the weighted sum.
+ * ------------------------------------------------------------------------ */
+AEOQ_API size_t aeoq_moe_fp8_block_workspace_size(int64_t T, int64_t top_k, int64_t num_experts, int64_t hidden,
+                                                  int64_t inter);
+AEOQ_API int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const void* top_k_index, int idx_dtype,
+                                        const float* top_k_weights, int64_t top_k, const uint8_t* gate_up,
+                                        const float* gate_up_scale, const uint8_t* down, const float* down_scale,
+                                        int64_t num_experts, int64_t hidden_dim, int64_t inter_dim, int activation,
+                                        void* out, void* workspace, size_t workspace_bytes, int* err_word,
+                                        void* stream);
 
 /* ------------------------------------------------------------------------
  * Self-test of the device division every quantized bit depends on: counts
