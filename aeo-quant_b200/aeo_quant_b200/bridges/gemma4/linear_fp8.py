@@ -102,3 +102,56 @@ class LinearFP8(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.bias is not None}, dtype=float8_e4m3fn")
+
+
+class LinearFP8Block(nn.Module):
+    """``nn.Linear`` with e4m3 weights that carry one f32 scale per 128 x 128
+    block, and activations quantized per 128 values of a row
+    (``gpu.fp8_block_matmul``). ``weight`` (out, in) float8_e4m3fn Parameter,
+    ``weight_scale`` (ceil(out/128), ceil(in/128)) float32 buffer, optional
+    bfloat16 ``bias``, added in f32 before the one rounding. ``in_features``
+    must be a multiple of 16; any ``out_features`` runs without padding.
+    Where a few large values share a row with small ones, a block's scale
+    holds them better than the row scales of :class:`LinearFP8`."""
+
+    weight: torch.Tensor
+    weight_scale: torch.Tensor
+    bias: torch.Tensor | None
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, device=None):
+        super().__init__()
+        if in_features % 16:
+            raise ValueError(f"in_features ({in_features}) must be a multiple of 16")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.weight = nn.Parameter(torch.empty(out_features, in_features, dtype=torch.float8_e4m3fn, device=device),
+                                   requires_grad=False)
+        self.register_buffer("weight_scale", torch.empty(-(-out_features // 128), -(-in_features // 128),
+                                                         dtype=torch.float32, device=device))
+        if bias:
+            self.bias = nn.Parameter(torch.empty(out_features, dtype=torch.bfloat16, device=device),
+                                     requires_grad=False)
+        else:
+            self.bias = None
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "LinearFP8Block":
+        """Quantize an existing ``nn.Linear`` on its device."""
+        from ...gpu.quant import quantize_2d_to_fp8_block
+
+        has_bias = linear.bias is not None
+        mod = cls(linear.in_features, linear.out_features, bias=has_bias, device="meta")
+        w_fp8, scale = quantize_2d_to_fp8_block(linear.weight.data)
+        mod.weight = nn.Parameter(w_fp8, requires_grad=False)
+        mod.weight_scale = scale
+        if has_bias:
+            mod.bias = nn.Parameter(linear.bias.data.to(torch.bfloat16), requires_grad=False)
+        return mod
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        from ...gpu.fp8_block_matmul import fp8_block_linear
+        return fp8_block_linear(x, self.weight, self.weight_scale, self.bias)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, dtype=float8_e4m3fn, block=128x128")

@@ -36,6 +36,13 @@ def _gemma4_experts_nvfp4_class_swap():
     return _swap(Gemma4TextExpertsNVFP4)
 
 
+def gemma4_experts_fp8_block_class_swap():
+    """Swap in ``Gemma4TextExpertsFP8Block`` (block-scaled FP8; not in the
+    reference)."""
+    from .modeling_fp8_block import Gemma4TextExpertsFP8Block
+    return _swap(Gemma4TextExpertsFP8Block)
+
+
 def _preconvert_fp8_scales(model):
     """(E, N, 1) bf16 scales -> (E, 1, N) fp32, in place (loader.py:47-64)."""
     from .modeling import Gemma4TextExpertsFP8
@@ -80,9 +87,12 @@ def _install_fused_routers(model):
 
 
 def load_gemma4(model_id_or_path, *, quant_format="fp8", **from_pretrained_kwargs):
-    """Dispatch by format (loader.py:67-76)."""
+    """Dispatch by format (loader.py:67-76); ``"fp8_block"`` is the
+    block-scaled FP8 format."""
     if quant_format == "nvfp4":
         return load_gemma4_nvfp4(model_id_or_path, **from_pretrained_kwargs)
+    if quant_format == "fp8_block":
+        return load_gemma4_fp8_block(model_id_or_path, **from_pretrained_kwargs)
     return load_gemma4_fp8(model_id_or_path, **from_pretrained_kwargs)
 
 
@@ -104,6 +114,41 @@ def load_gemma4_nvfp4(model_id_or_path, **from_pretrained_kwargs):
     with _gemma4_experts_nvfp4_class_swap():
         model = _from_pretrained(model_id_or_path, from_pretrained_kwargs)
     return _install_fused_routers(model)
+
+
+def load_gemma4_fp8_block(model_id_or_path, **from_pretrained_kwargs):
+    """Load a checkpoint with block-scaled FP8 experts (``save_pretrained``
+    of a model that ``quantize_experts_to_fp8_block`` converted) under the
+    class swap. On a GPU the routers get the fused forward as well."""
+    with gemma4_experts_fp8_block_class_swap():
+        model = _from_pretrained(model_id_or_path, from_pretrained_kwargs)
+    return _install_fused_routers(model)
+
+
+@torch.no_grad()
+def quantize_experts_to_fp8_block(model):
+    """Replace every bf16 ``Gemma4TextExperts`` in ``model`` by a
+    ``Gemma4TextExpertsFP8Block`` holding its block-scaled FP8 quantization
+    (``quantize_3d_to_fp8_block``), on the experts' device, one layer at a
+    time. Returns the number of modules converted."""
+    from ...gpu.quant import quantize_3d_to_fp8_block
+    from .modeling_fp8_block import Gemma4TextExpertsFP8Block
+
+    targets = []
+    for _, mod in model.named_modules():
+        for child_name, child in mod.named_children():
+            if type(child) is modeling_gemma4.Gemma4TextExperts:
+                targets.append((mod, child_name, child))
+    for parent, child_name, old in targets:
+        with torch.device("meta"):
+            new = Gemma4TextExpertsFP8Block(_ExpertShape(old))
+        for proj in ("gate_up_proj", "down_proj"):
+            q, scale = quantize_3d_to_fp8_block(getattr(old, proj).detach())
+            setattr(new, proj, torch.nn.Parameter(q, requires_grad=False))
+            setattr(new, f"{proj}_scale", scale)
+        setattr(parent, child_name, new)
+        del old
+    return len(targets)
 
 
 @torch.no_grad()
