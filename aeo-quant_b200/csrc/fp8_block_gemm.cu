@@ -12,15 +12,14 @@
 // buffers, so the scaling of block b runs under the MMAs of block b + 1.
 // Tokens are the MMA's 128 rows: a TMEM lane is a token and a thread owns
 // one token, so its scale sa is one value per block and sw is the same for a
-// whole run of columns: the scaling is one packed f32 fma per two sums.
+// whole run of columns: the scaling is one f32 fma per sum.
 //
 //   warp 0      TMA: per 128-wide K step one tile of a and one of w
 //               (128-byte swizzle)
-//   warp 1      TMEM owner and MMA issuer
+//   warps 1-2   MMA issuers (warp 1 owns the TMEM)
 //   warps 4-11  scaling and epilogue: two warps per TMEM lane quadrant, each
-//               with half of the columns (128 f32 sums per thread: the two
-//               other warps only exist so that setmaxnreg can give their
-//               registers to these)
+//               with half of the columns (128 f32 sums per thread; setmaxnreg
+//               gives them registers of warps 0-3)
 //
 // One CTA per SM walks the tiles, output features fastest (they share the
 // tile of a in L2).
@@ -63,6 +62,7 @@ struct FbParams {
   int tiles_n;
   void* out; int out_dt; int64_t ldc;   // store: row stride in elements
   const __nv_bfloat16* bias;            // store: N values or null
+  bool out_tma;           // bf16 tiles leave through shared memory and TMA
   int64_t I;              // GLU: gate rows are w rows [0, I), up rows [I, 2 I)
   int act;
   uint8_t* hq; int64_t hq_ld;           // GLU: quantized h rows
@@ -70,9 +70,12 @@ struct FbParams {
   int* err;
 };
 
-template <int BN>
+template <int BN, int EPI>
 struct FbLayout {
   static constexpr uint32_t kA = 128 * 128, kB = BN * 128, kStage = kA + kB;
+  // a bf16 tile on its way out (store epilogue): boxes of 128 rows x 64
+  // columns, 128-byte swizzle
+  static constexpr uint32_t kOut = EPI == kFbStore ? 128 * BN * 2 : 0;
   struct Ctl {
     uint64_t full[kFbMaxStages], empty[kFbMaxStages];
     uint64_t acc_full[2], acc_empty[2];
@@ -80,8 +83,8 @@ struct FbLayout {
     float amax[2][128];                // GLU: the two column halves' maxima per row
     int tile_off[kFbMaxExperts + 1];
   };
-  static constexpr int kStages = std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl)) / (int)kStage);
-  static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + sizeof(Ctl);
+  static constexpr int kStages = std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl) - (int)kOut) / (int)kStage);
+  static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + kOut + sizeof(Ctl);
   static constexpr uint32_t kTmemCols = 2 * BN;
 };
 
@@ -91,13 +94,13 @@ struct FbTile {
 };
 
 template <int BN, int EPI>
-__device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off, int64_t t) {
+__device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off, int t) {
   FbTile r;
-  const int64_t mt = t / p.tiles_n;
-  r.n0 = (t - mt * p.tiles_n) * (EPI == kFbGlu ? BN / 2 : BN);
+  const int mt = t / p.tiles_n;
+  r.n0 = (int64_t)(t - mt * p.tiles_n) * (EPI == kFbGlu ? BN / 2 : BN);
   if (!p.grp_off) {
     r.expert = 0;
-    r.row0 = mt * 128;
+    r.row0 = (int64_t)mt * 128;
     r.rows = (int)min((int64_t)128, p.M - r.row0);
     return r;
   }
@@ -107,26 +110,9 @@ __device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off
     if (tile_off[mid] <= mt) lo = mid; else hi = mid;
   }
   r.expert = lo;
-  const int64_t in = (mt - tile_off[lo]) * 128;
-  const int64_t g0 = __ldg(p.grp_off + lo), g1 = __ldg(p.grp_off + lo + 1);
-  r.row0 = g0 + in;
-  r.rows = (int)min((int64_t)128, g1 - r.row0);
-  return r;
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-  return d;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  const int g0 = __ldg(p.grp_off + lo), g1 = __ldg(p.grp_off + lo + 1);
+  r.row0 = g0 + (mt - tile_off[lo]) * 128;
+  r.rows = min(128, g1 - (int)r.row0);
   return r;
 }
 
@@ -143,11 +129,12 @@ __device__ __forceinline__ float fb_act(int act, float x) {
 template <int BN, int EPI>
 __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                       const __grid_constant__ CUtensorMap tmW,
+                                                                      const __grid_constant__ CUtensorMap tmO,
                                                                       const FbParams p) {
-  using L = FbLayout<BN>;
+  using L = FbLayout<BN, EPI>;
   extern __shared__ __align__(1024) uint8_t dsmem[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
-  auto* sh = reinterpret_cast<typename L::Ctl*>(base + L::kStages * L::kStage);
+  auto* sh = reinterpret_cast<typename L::Ctl*>(base + L::kStages * L::kStage + L::kOut);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -162,6 +149,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     sm100::fence_barrier_init();
     sm100::prefetch_tmap(&tmA);
     sm100::prefetch_tmap(&tmW);
+    if (EPI == kFbStore && p.out_tma) sm100::prefetch_tmap(&tmO);
   }
   if (p.grp_off)
     for (int e = tid; e <= p.E; e += kFbThreads) sh->tile_off[e] = p.tile_off[e];
@@ -170,7 +158,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const int64_t total = (p.grp_off ? (int64_t)sh->tile_off[p.E] : p.tiles_m) * p.tiles_n;
+  const int total = (p.grp_off ? sh->tile_off[p.E] : (int)p.tiles_m) * p.tiles_n;
   const int KB = p.KB;
 
   if (warp < 4) {
@@ -180,7 +168,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     const bool leader = sm100::elect_one();
     uint32_t g = 0;      // K steps so far
     bool alive = true;
-    for (int64_t t = blockIdx.x; t < total && alive; t += gridDim.x) {
+    for (int t = blockIdx.x; t < total && alive; t += gridDim.x) {
       const FbTile ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
       const int64_t w0 = ti.expert * p.N + ti.n0;
       for (int kb = 0; kb < KB; ++kb, ++g) {
@@ -197,30 +185,33 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         __syncwarp();
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp < 3) {
+    // ------------------------------------------------------------ MMA issuers
+    // Warp 1 takes the even K steps and TMEM buffer 0, warp 2 the odd ones.
+    // A wait that is already satisfied costs its thread about 100 cycles; two
+    // issuers spend them under one another's MMAs (one: 606 cycles per step
+    // with two waits, against the MMAs' 512).
     const bool leader = sm100::elect_one();
     constexpr uint32_t idesc = sm100::idesc_f8(BN);
-    uint32_t g = 0;
-    bool alive = true;
-    for (int64_t t = blockIdx.x; t < total && alive; t += gridDim.x) {
-      for (int kb = 0; kb < KB; ++kb, ++g) {
-        const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
-        const uint32_t b = g & 1, bph = (g >> 1) & 1;
-        if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72) ||
-            !sm100::mbar_wait(&sh->full[s], ph, p.err, 73)) { alive = false; break; }
-        sm100::tc_fence_after();
-        if (leader) {
-          const uint32_t sa = sm100::smem_u32(base + s * L::kStage), sb = sa + L::kA;
+    const uint32_t b = warp - 1;
+    const int mine = (int)blockIdx.x < total ? (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+    const uint32_t steps = (uint32_t)mine * KB;
+    for (uint32_t g = b; g < steps; g += 2) {
+      const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1, bph = (g >> 1) & 1;
+      if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72) ||
+          !sm100::mbar_wait(&sh->full[s], ph, p.err, 73))
+        break;
+      sm100::tc_fence_after();
+      if (leader) {
+        const uint32_t sa = sm100::smem_u32(base + s * L::kStage), sb = sa + L::kA;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sm100::tc_mma_f8(tmem + b * BN, sm100::sdesc_k_sw128(sa + 32 * j), sm100::sdesc_k_sw128(sb + 32 * j),
-                             idesc, j ? 1u : 0u);
-          sm100::tc_commit(&sh->empty[s]);
-          sm100::tc_commit(&sh->acc_full[b]);
-        }
-        __syncwarp();
+        for (int j = 0; j < 4; ++j)
+          sm100::tc_mma_f8(tmem + b * BN, sm100::sdesc_k_sw128(sa + 32 * j), sm100::sdesc_k_sw128(sb + 32 * j), idesc,
+                           j ? 1u : 0u);
+        sm100::tc_commit(&sh->empty[s]);
+        sm100::tc_commit(&sh->acc_full[b]);
       }
+      __syncwarp();
     }
   }
   } else {
@@ -241,32 +232,41 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     // A warp whose wait ran out goes through its remaining tiles without
     // waiting or storing: the other warps count on it at the barriers below.
     bool alive = true;
-    for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-      const FbTile ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
-      const bool live = row < ti.rows;
-      const float* sa = p.sa + (ti.row0 + (live ? row : 0)) * KB;
-      const float *sw0, *sw1;
-      {
-        const float* se = p.sw + ti.expert * p.NB * KB;
-        // a run of columns that lies past the last row of w reads the last
-        // scale; its sums are not used
-        const int64_t c0 = min(ti.n0 + col_of(0), p.N - 1);
-        const int64_t c1 = EPI == kFbGlu ? min(p.I + ti.n0 + half * (BN / 4), p.N - 1) : c0;
-        sw0 = se + (c0 / kFbBlock) * KB;
-        sw1 = se + (c1 / kFbBlock) * KB;
-      }
-      uint64_t acc[kCols / 2];
+    FbTile ti{};
+    const float *sa = p.sa, *sw0 = p.sw, *sw1 = p.sw;
+    float a = 0.0f, w0 = 0.0f, w1 = 0.0f;
+    // a tile's scales: pointers, and the values of its first K step
+    auto open_tile = [&](int t) {
+      ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
+      sa = p.sa + (ti.row0 + (row < ti.rows ? row : 0)) * KB;
+      const float* se = p.sw + ti.expert * p.NB * KB;
+      // a run of columns that lies past the last row of w reads the last
+      // scale; its sums are not used
+      const int64_t c0 = min(ti.n0 + col_of(0), p.N - 1);
+      const int64_t c1 = EPI == kFbGlu ? min(p.I + ti.n0 + half * (BN / 4), p.N - 1) : c0;
+      sw0 = se + (c0 / kFbBlock) * KB;
+      sw1 = se + (c1 / kFbBlock) * KB;
+      a = __ldg(sa);
+      w0 = __ldg(sw0);
+      w1 = __ldg(sw1);
+    };
+    if ((int)blockIdx.x < total) open_tile(blockIdx.x);
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      if (!alive) open_tile(t);      // (a live warp opened it in the last K step of the tile before)
+      const FbTile cur = ti;
+      const bool live = row < cur.rows;
+      float acc[kCols];
 #pragma unroll
-      for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
-      float a = __ldg(sa), w0 = __ldg(sw0), w1 = __ldg(sw1);
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
       for (int kb = 0; kb < KB; ++kb, ++g) {
         const uint32_t b = g & 1, bph = (g >> 1) & 1;
         const float c0 = a * w0, c1 = a * w1;
-        const uint64_t cc0 = pack2(c0, c0), cc1 = pack2(c1, c1);
         if (kb + 1 < KB) {
           a = __ldg(sa + kb + 1);
           w0 = __ldg(sw0 + kb + 1);
           w1 = __ldg(sw1 + kb + 1);
+        } else if (t + (int)gridDim.x < total) {
+          open_tile(t + gridDim.x);
         }
         if (!alive || !sm100::mbar_wait(&sh->acc_full[b], bph, p.err, 74)) {
           alive = false;
@@ -274,37 +274,67 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         }
         sm100::tc_fence_after();
         const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
+        // the read of a chunk of 32 columns runs under the sums of the last
+        uint32_t r[2][32];
+        sm100::tmem_ld32_nowait(tq + col_of(0), r[0]);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          uint32_t r[32];
-          sm100::tmem_ld32_nowait(tq + col_of(c), r);
           sm100::tmem_ld_wait();
-          if (c == kChunks - 1) {
+          if (c + 1 < kChunks) {
+            sm100::tmem_ld32_nowait(tq + col_of(c + 1), r[(c + 1) & 1]);
+          } else {
             sm100::tc_fence_before();
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&sh->acc_empty[b]);
           }
-          const uint64_t cc = (EPI == kFbGlu && c >= kChunks / 2) ? cc1 : cc0;
+          const float cs = (EPI == kFbGlu && c >= kChunks / 2) ? c1 : c0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[16 * c + i] =
-                fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), cc, acc[16 * c + i]);
+          for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), cs, acc[32 * c + i]);
         }
       }
       if constexpr (EPI == kFbStore) {
-        if (!live || !alive) continue;
-        const int64_t n0 = ti.n0 + half * kCols;
-        const int64_t o = (ti.row0 + row) * p.ldc + n0;
+        const int64_t n0 = cur.n0 + half * kCols;
+        const int64_t o = (cur.row0 + row) * p.ldc + n0;
         if (p.bias) {
 #pragma unroll
-          for (int i = 0; i < kCols / 2; ++i) {
-            const float2 v = unpack2(acc[i]);
-            const float b0 = n0 + 2 * i < p.N ? __bfloat162float(p.bias[n0 + 2 * i]) : 0.0f;
-            const float b1 = n0 + 2 * i + 1 < p.N ? __bfloat162float(p.bias[n0 + 2 * i + 1]) : 0.0f;
-            acc[i] = pack2(v.x + b0, v.y + b1);
-          }
+          for (int i = 0; i < kCols; ++i) acc[i] += n0 + i < p.N ? __bfloat162float(p.bias[n0 + i]) : 0.0f;
         }
         const int64_t left = p.N - n0;     // columns of this thread that exist
+        // Through shared memory: a thread's row in pieces of 16 bytes, placed
+        // so that 8 lanes fill 8 different bank groups; one TMA store per 64
+        // columns then writes whole rows of 128 bytes (stored directly, the
+        // 32 rows of a warp's store are 32 half sectors: 53 us of 211 at M =
+        // 32768, N = 1408, K = 2816). Only whole row tiles: behind a
+        // shorter one lie another expert's rows. TMA itself stops at row M
+        // and column N.
+        if (p.out_tma && (cur.rows == 128 || !p.grp_off)) {
+          uint8_t* box = base + L::kStages * L::kStage + half * (128 * kCols * 2);
+          const int id = 2 + half;
+          if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+#pragma unroll
+          for (int i = 0; i < kCols / 8; ++i) {
+            __align__(16) __nv_bfloat162 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(acc[8 * i + 2 * j], acc[8 * i + 2 * j + 1]);
+            *reinterpret_cast<uint4*>(box + (i / 8) * 16384 + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
+                *reinterpret_cast<const uint4*>(v);
+          }
+          sm100::fence_proxy_async_smem();
+          asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+          if (row == 0 && alive) {
+#pragma unroll
+            for (int x = 0; x < kCols / 64; ++x)
+              if (64 * x < left)
+                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                 reinterpret_cast<uint64_t>(&tmO)),
+                             "r"((int)((n0 + 64 * x) * 2)), "r"((int)cur.row0), "r"(sm100::smem_u32(box + x * 16384))
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          continue;
+        }
+        if (!live || !alive) continue;
         if (p.out_dt == AEOQ_BF16) {
           __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + o;
           const bool wide = p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
@@ -312,10 +342,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           for (int i = 0; i < kCols / 8; ++i) {
             __align__(16) __nv_bfloat162 v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack2(acc[4 * i + j]);
-              v[j] = __floats2bfloat162_rn(f.x, f.y);
-            }
+            for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(acc[8 * i + 2 * j], acc[8 * i + 2 * j + 1]);
             if (wide && 8 * i + 8 <= left) {
               *reinterpret_cast<uint4*>(d + 8 * i) = *reinterpret_cast<const uint4*>(v);
             } else {
@@ -329,14 +356,13 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           const bool wide = p.ldc % 4 == 0 && (uintptr_t)p.out % 16 == 0;
 #pragma unroll
           for (int i = 0; i < kCols / 4; ++i) {
-            const float2 u = unpack2(acc[2 * i]), v = unpack2(acc[2 * i + 1]);
             if (wide && 4 * i + 4 <= left) {
-              *reinterpret_cast<float4*>(d + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
+              *reinterpret_cast<float4*>(d + 4 * i) =
+                  make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
             } else {
-              if (4 * i < left) d[4 * i] = u.x;
-              if (4 * i + 1 < left) d[4 * i + 1] = u.y;
-              if (4 * i + 2 < left) d[4 * i + 2] = v.x;
-              if (4 * i + 3 < left) d[4 * i + 3] = v.y;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (4 * i + j < left) d[4 * i + j] = acc[4 * i + j];
             }
           }
         }
@@ -344,17 +370,14 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         // h = act(gate) * up of this thread's BN / 4 columns; columns past I
         // (and rows past the tile's) count as zeros
         constexpr int kH = BN / 4;
-        const int64_t n0 = ti.n0 + half * kH;
+        const int64_t n0 = cur.n0 + half * kH;
         const int n_ok = (int)min((int64_t)kH, p.I - n0);
         float h[kH];
         uint32_t key = 0;
 #pragma unroll
-        for (int i = 0; i < kH / 2; ++i) {
-          const float2 gt = unpack2(acc[i]), up = unpack2(acc[kH / 2 + i]);
-          h[2 * i] = 2 * i < n_ok ? fb_act(p.act, gt.x) * up.x : 0.0f;
-          h[2 * i + 1] = 2 * i + 1 < n_ok ? fb_act(p.act, gt.y) * up.y : 0.0f;
-          key = max(key, __float_as_uint(h[2 * i]) & 0x7FFFFFFFu);
-          key = max(key, __float_as_uint(h[2 * i + 1]) & 0x7FFFFFFFu);
+        for (int i = 0; i < kH; ++i) {
+          h[i] = i < n_ok ? fb_act(p.act, acc[i]) * acc[kH + i] : 0.0f;
+          key = max(key, __float_as_uint(h[i]) & 0x7FFFFFFFu);
         }
         sh->amax[half][row] = __uint_as_float(key);
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kFbEpiWarps) : "memory");
@@ -363,8 +386,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kFbEpiWarps) : "memory");
         const float2 s = fb_scales(__uint_as_float(key));
         if (live && alive) {
-          if (half == 0) p.hs[(ti.row0 + row) * p.hs_ld + ti.n0 / kFbBlock] = s.y;
-          uint8_t* d = p.hq + (ti.row0 + row) * p.hq_ld + n0;
+          if (half == 0) p.hs[(cur.row0 + row) * p.hs_ld + cur.n0 / kFbBlock] = s.y;
+          uint8_t* d = p.hq + (cur.row0 + row) * p.hq_ld + n0;
 #pragma unroll
           for (int i = 0; i < kH / 16; ++i) {
             if (16 * i >= n_ok) break;
@@ -380,6 +403,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
       }
     }
   }
+  // the stores' reads of shared memory are over before it goes away
+  if (EPI == kFbStore && warp >= 4) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   sm100::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -389,18 +414,25 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
 }
 
 template <int BN, int EPI>
-static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, const FbParams& p, int64_t max_tiles,
+static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbParams p, int64_t max_tiles,
                        cudaStream_t st) {
-  using L = FbLayout<BN>;
-  CUtensorMap ta, tw;
+  using L = FbLayout<BN, EPI>;
+  CUtensorMap ta, tw, to;
   int rc = make_tmap_bytes(&ta, a, a_rows, p.K, p.K, 128, 128, true);
   if (rc) return rc;
   rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, EPI == kFbGlu ? BN / 2 : BN, true);
   if (rc) return rc;
+  to = ta;
+  p.out_tma = EPI == kFbStore && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+  if (p.out_tma) {
+    rc = make_tmap_bytes(&to, p.out, p.M, p.N * 2, p.ldc * 2, 128, 128, true);
+    if (rc) return rc;
+  }
+  AEOQ_REQUIRE(max_tiles <= 0x7FFFFFFF, AEOQ_ERR_INVALID, "fp8_block_gemm: too many tiles");
   rc = func_smem_attr((const void*)fp8_block_gemm_kernel<BN, EPI>, L::kBytes, -1, "fp8_block_gemm");
   if (rc) return rc;
   const int ctas = (int)std::min<int64_t>(device_sm_count(), max_tiles);
-  fp8_block_gemm_kernel<BN, EPI><<<ctas, kFbThreads, L::kBytes, st>>>(ta, tw, p);
+  fp8_block_gemm_kernel<BN, EPI><<<ctas, kFbThreads, L::kBytes, st>>>(ta, tw, to, p);
   return check_launch("fp8_block_gemm_kernel");
 }
 
