@@ -65,7 +65,8 @@ __device__ __forceinline__ uint2 fb_codes8(const float (&v)[8], float inv) {
                     fb_codes4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
 }
 
-// Rows [0, rows) of x (or x[idx[r]], r < *n_rows) quantized per 128 values.
+// Rows [0, rows) of x (or x[idx[r]], r < *n_rows) quantized per 128 values; their
+// scales (rows, ceil(K / 128)).
 int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, const int* idx,
                      const int* n_rows, uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st);
 

@@ -54,7 +54,8 @@ struct FbParams {
   int K, KB;              // K and its blocks
   int64_t NB;             // scale rows per expert, ceil(N / 128)
   int E;
-  const float* sa;        // (rows of a, KB)
+  const float* sa;        // (rows of a, KB): a row's scales share lines that stay in L1 for several K
+                          // steps (the other order, 8192 x 8192 x 8192: 689 against 521 us)
   const float* sw;        // (E, NB, KB)
   const int* grp_off;     // grouped: rows [grp_off[e], grp_off[e + 1]) are expert e's; null: dense
   const int* tile_off;    // grouped: row tiles before expert e's, E + 1 values
@@ -62,7 +63,7 @@ struct FbParams {
   int tiles_n;
   void* out; int out_dt; int64_t ldc;   // store: row stride in elements
   const __nv_bfloat16* bias;            // store: N values or null
-  bool out_tma;           // bf16 tiles leave through shared memory and TMA
+  bool out_tma;           // whole tiles may leave by TMA
   int64_t I;              // GLU: gate rows are w rows [0, I), up rows [I, 2 I)
   int act;
   uint8_t* hq; int64_t hq_ld;           // GLU: quantized h rows
@@ -73,10 +74,8 @@ struct FbParams {
 template <int BN, int EPI>
 struct FbLayout {
   static constexpr uint32_t kA = 128 * 128, kB = BN * 128, kStage = kA + kB;
-  // a bf16 tile on its way out (store epilogue): boxes of 128 rows x 64
-  // columns, 128-byte swizzle. Not with 256 columns, where it would cost a
-  // stage: those tiles serve experts with few rows, which store directly.
-  static constexpr uint32_t kOut = EPI == kFbStore && BN == 128 ? 128 * BN * 2 : 0;
+  // the tile on its way out as bf16 (store epilogue)
+  static constexpr uint32_t kOut = EPI == kFbStore ? 128 * BN * 2 : 0;
   struct Ctl {
     uint64_t full[kFbMaxStages], empty[kFbMaxStages];
     uint64_t acc_full[2], acc_empty[2];
@@ -84,12 +83,9 @@ struct FbLayout {
     float amax[2][128];                // GLU: the two column halves' maxima per row
     int tile_off[kFbMaxExperts + 1];
   };
-  // An even number: the K steps of one parity, and with them the ring's slots
-  // of that parity, belong to one issuer. (A parity wait is only sound where
-  // its waiter holds back the barrier's next phase.)
   static constexpr int kStages =
-      std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl) - (int)kOut) / (int)kStage) / 2 * 2;
-  static_assert(kStages >= 4, "the ring needs four stages");
+      std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl) - (int)kOut) / (int)kStage);
+  static_assert(kStages >= 3, "the ring needs three stages");
   static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + kOut + sizeof(Ctl);
   static constexpr uint32_t kTmemCols = 2 * BN;
 };
@@ -99,11 +95,22 @@ struct FbTile {
   int rows;                   // valid rows
 };
 
+// Row and column tile of tile number t. Columns go fastest; where the last
+// column of tiles is short (`half_last`: no second column half) its tiles,
+// which take half as long, come after all others, so that they fill the
+// CTAs' uneven ends.
+__device__ __forceinline__ int2 fb_place(int t, int tiles_m, int tiles_n, bool half_last) {
+  const int wide = tiles_n - (int)half_last, n_wide = tiles_m * wide;
+  if (t >= n_wide) return make_int2(t - n_wide, tiles_n - 1);
+  const int mt = t / wide;
+  return make_int2(mt, t - mt * wide);
+}
+
 template <int BN, int EPI>
-__device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off, int t) {
+__device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off, int2 at) {
   FbTile r;
-  const int mt = t / p.tiles_n;
-  r.n0 = (int64_t)(t - mt * p.tiles_n) * (EPI == kFbGlu ? BN / 2 : BN);
+  const int mt = at.x;
+  r.n0 = (int64_t)at.y * (EPI == kFbGlu ? BN / 2 : BN);
   if (!p.grp_off) {
     r.expert = 0;
     r.row0 = (int64_t)mt * 128;
@@ -137,81 +144,85 @@ __device__ __forceinline__ float fb_act(int act, float x) {
 // share them. `row` is the thread's row in its 128-row tile; four warps hold
 // one half.
 
-// bf16 or f32 store of kCols columns from cur.n0 + kCols * half on.
+// Store of a whole 128-row tile's kCols bf16 columns from cur.n0 + kCols *
+// half on: through shared memory (a thread's row in pieces of 16 bytes, placed
+// so that 8 lanes fill 8 different bank groups) and one TMA store per 64
+// columns, which stops at row M and column N by itself. Stored directly, the
+// 32 rows of a warp's store are 32 half sectors: 53 us of 211 at M = 32768, N
+// = 1408, K = 2816. The kernel gives a stage of its ring for the room (with
+// half of it, used twice, the second half waits for the first: 161 us
+// against 145).
 template <int kCols>
-__device__ __forceinline__ void fb_store_half(const FbParams& p, const CUtensorMap& tmO, const FbTile& cur,
-                                              uint8_t* box, float (&acc)[kCols], int row, int half, bool alive) {
-  const bool live = row < cur.rows;
+__device__ __forceinline__ void fb_store_tile(const FbParams& p, const CUtensorMap& tmO, const FbTile& cur,
+                                              uint8_t* box, const float (&acc)[kCols], int row, int half, bool alive) {
   const int64_t n0 = cur.n0 + half * kCols;
-  const int64_t o = (cur.row0 + row) * p.ldc + n0;
-  if (p.bias) {
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) acc[i] += n0 + i < p.N ? __bfloat162float(p.bias[n0 + i]) : 0.0f;
+  for (int i = 0; i < kCols / 8; ++i) {
+    __align__(16) __nv_bfloat162 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(acc[8 * i + 2 * j], acc[8 * i + 2 * j + 1]);
+    *reinterpret_cast<uint4*>(box + (i / 8) * 16384 + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
+        *reinterpret_cast<const uint4*>(v);
   }
-  const int64_t left = p.N - n0;     // columns of this thread that exist
-  // Through shared memory: a thread's row in pieces of 16 bytes, placed so
-  // that 8 lanes fill 8 different bank groups; one TMA store per 64 columns
-  // then writes whole rows of 128 bytes (stored directly, the 32 rows of a
-  // warp's store are 32 half sectors: 53 us of 211 at M = 32768, N = 1408,
-  // K = 2816). Only whole row tiles: behind a shorter one lie another
-  // expert's rows. TMA itself stops at row M and column N.
-  if (p.out_tma && (cur.rows == 128 || !p.grp_off)) {
-    const int id = 2 + half;
-    if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+  sm100::fence_proxy_async_smem();
+  asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+  if (row == 0 && alive) {
 #pragma unroll
-    for (int i = 0; i < kCols / 8; ++i) {
-      __align__(16) __nv_bfloat162 v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(acc[8 * i + 2 * j], acc[8 * i + 2 * j + 1]);
-      *reinterpret_cast<uint4*>(box + (i / 8) * 16384 + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
-          *reinterpret_cast<const uint4*>(v);
-    }
-    sm100::fence_proxy_async_smem();
-    asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
-    if (row == 0 && alive && cur.rows > 0) {
-#pragma unroll
-      for (int x = 0; x < kCols / 64; ++x)
-        if (64 * x < left)
-          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                           reinterpret_cast<uint64_t>(&tmO)),
-                       "r"((int)((n0 + 64 * x) * 2)), "r"((int)cur.row0), "r"(sm100::smem_u32(box + x * 16384))
-                       : "memory");
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    }
-    return;
+    for (int x = 0; x < kCols / 64; ++x)
+      if (n0 + 64 * x < p.N)
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                         reinterpret_cast<uint64_t>(&tmO)),
+                     "r"((int)((n0 + 64 * x) * 2)), "r"((int)cur.row0), "r"(sm100::smem_u32(box + x * 16384))
+                     : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
-  if (!live || !alive) return;
-  if (p.out_dt == AEOQ_BF16) {
-    __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + o;
-    const bool wide = p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+}
+
+// The other tiles (behind a short one lie another expert's rows; f32; rows
+// that are not 16-byte aligned), rows and columns left out one by one: each
+// warp turns its 32 rows around in 4 KB of shared memory, 128 bytes of a row
+// at a time, so that a store instruction writes four whole lines.
+template <class T, int kCols>
+__device__ __forceinline__ void fb_store_rows(const FbParams& p, const FbTile& cur, uint8_t* box,
+                                              const float (&acc)[kCols], int q, int half, bool alive) {
+  constexpr int kPer = 16 / (int)sizeof(T), kRound = 8 * kPer;     // columns per piece, per round
+  const int lane = threadIdx.x & 31;
+  const int64_t n0 = cur.n0 + half * kCols;
+  const bool wide = p.ldc % kPer == 0 && (uintptr_t)p.out % 16 == 0;
+  const int sub = lane >> 3, ch = lane & 7;
+  T* out = reinterpret_cast<T*>(p.out) + (cur.row0 + 32 * q + sub) * p.ldc + n0 + ch * kPer;
+  const int rows = alive ? cur.rows - 32 * q - sub : 0;            // row 4 j exists if 4 j < rows
 #pragma unroll
-    for (int i = 0; i < kCols / 8; ++i) {
-      __align__(16) __nv_bfloat162 v[4];
+  for (int x = 0; x < kCols / kRound; ++x) {
+    const int64_t left = p.N - n0 - x * kRound - ch * kPer;        // columns from this lane's piece on
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(acc[8 * i + 2 * j], acc[8 * i + 2 * j + 1]);
-      if (wide && 8 * i + 8 <= left) {
-        *reinterpret_cast<uint4*>(d + 8 * i) = *reinterpret_cast<const uint4*>(v);
+    for (int i = 0; i < 8; ++i) {
+      const float* f = acc + x * kRound + i * kPer;
+      __align__(16) T v[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if constexpr (sizeof(T) == 2) v[j] = __float2bfloat16_rn(f[j]);
+        else v[j] = f[j];
+      }
+      *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(v);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (4 * j >= rows || left <= 0) continue;
+      const int r = 4 * j + sub;
+      const uint4 u = *reinterpret_cast<const uint4*>(box + r * 128 + ((ch ^ (r & 7)) << 4));
+      T* d = out + (int64_t)(4 * j) * p.ldc + x * kRound;
+      if (wide && left >= kPer) {
+        *reinterpret_cast<uint4*>(d) = u;
       } else {
+        const T* v = reinterpret_cast<const T*>(&u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (8 * i + j < left) d[8 * i + j] = j & 1 ? v[j / 2].y : v[j / 2].x;
+        for (int k = 0; k < kPer; ++k)
+          if (k < left) d[k] = v[k];
       }
     }
-  } else {
-    float* d = reinterpret_cast<float*>(p.out) + o;
-    const bool wide = p.ldc % 4 == 0 && (uintptr_t)p.out % 16 == 0;
-#pragma unroll
-    for (int i = 0; i < kCols / 4; ++i) {
-      if (wide && 4 * i + 4 <= left) {
-        *reinterpret_cast<float4*>(d + 4 * i) =
-            make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (4 * i + j < left) d[4 * i + j] = acc[4 * i + j];
-      }
-    }
+    __syncwarp();
   }
 }
 
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
   if (tid == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       sm100::mbar_init(&sh->full[s], 1);
-      sm100::mbar_init(&sh->empty[s], 1);
+      sm100::mbar_init(&sh->empty[s], 2);      // both issuers
     }
     for (int b = 0; b < 2; ++b) {
       sm100::mbar_init(&sh->acc_full[b], 1);
@@ -280,13 +291,19 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
   }
   if (p.grp_off)
     for (int e = tid; e <= p.E; e += kFbThreads) sh->tile_off[e] = p.tile_off[e];
+  const int* tile_off = sh->tile_off;
   if (warp == 1) sm100::tmem_alloc(&sh->tmem_base, L::kTmemCols);
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const int total = (p.grp_off ? sh->tile_off[p.E] : (int)p.tiles_m) * p.tiles_n;
+  const int tiles_m = p.grp_off ? tile_off[p.E] : (int)p.tiles_m, total = tiles_m * p.tiles_n;
   const int KB = p.KB;
+  // Does the second column half of the tile at column n0 exist? Where it does
+  // not, its MMAs, sums and stores are left out.
+  auto has_two = [&](int64_t n0) { return EPI == kFbGlu ? n0 + BN / 4 < p.I : n0 + BN / 2 < p.N; };
+  const bool half_last = !has_two((int64_t)(p.tiles_n - 1) * (EPI == kFbGlu ? BN / 2 : BN));
+  auto place = [&](int t) { return fb_place(t, tiles_m, p.tiles_n, half_last); };
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFbRegsLow));
@@ -296,7 +313,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     uint32_t g = 0;      // K steps so far
     bool alive = true;
     for (int t = blockIdx.x; t < total && alive; t += gridDim.x) {
-      const FbTile ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
+      const FbTile ti = fb_tile<BN, EPI>(p, tile_off, place(t));
       const int64_t w0 = ti.expert * p.N + ti.n0;
       for (int kb = 0; kb < KB; ++kb, ++g) {
         const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
@@ -305,26 +322,47 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           uint8_t* st = base + s * L::kStage;
           sm100::mbar_arrive_expect_tx(&sh->full[s], L::kStage);
           sm100::tma_load_2d(st, &tmA, kb * 128, (int32_t)ti.row0, &sh->full[s]);
-          sm100::tma_load_2d(st + L::kA, &tmW, kb * 128, (int32_t)w0, &sh->full[s]);
-          if constexpr (EPI == kFbGlu)
-            sm100::tma_load_2d(st + L::kA + L::kB / 2, &tmW, kb * 128, (int32_t)(w0 + p.I), &sh->full[s]);
+          if constexpr (EPI == kFbGlu) {
+            // per half: its gate rows, then the up rows that go with them
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sm100::tma_load_2d(st + L::kA + i * (L::kB / 4), &tmW, kb * 128,
+                                 (int32_t)(w0 + (i >> 1) * (BN / 4) + (i & 1) * p.I), &sh->full[s]);
+          } else {
+            sm100::tma_load_2d(st + L::kA, &tmW, kb * 128, (int32_t)w0, &sh->full[s]);
+          }
         }
         __syncwarp();
       }
     }
   } else if (warp < 3) {
     // ------------------------------------------------------------ MMA issuers
-    // Warp 1 takes the even K steps and TMEM buffer 0, warp 2 the odd ones.
-    // A wait that is already satisfied costs its thread about 100 cycles; two
-    // issuers spend them under one another's MMAs (one: 606 cycles per step
-    // with two waits, against the MMAs' 512).
+    // Warp 1 takes the even K steps and TMEM buffer 0, warp 2 the odd ones:
+    // a wait costs its thread about 100 cycles even when it is already
+    // satisfied, and two issuers spend them under one another's MMAs (one, with
+    // its two waits a step: 606 cycles per step against the MMAs' 512). A parity
+    // wait is only sound where its waiter holds back the barrier's next phase,
+    // so both look at every stage and both give it back.
     const bool leader = sm100::elect_one();
-    constexpr uint32_t idesc = sm100::idesc_f8(BN);
     const uint32_t b = warp - 1;
     const int mine = (int)blockIdx.x < total ? (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
     const uint32_t steps = (uint32_t)mine * KB;
-    for (uint32_t g = b; g < steps; g += 2) {
+    int t = blockIdx.x, kb = 0;          // tile and K step of g
+    uint32_t idesc = 0;
+    for (uint32_t g = 0; g < steps; ++g, ++kb) {
+      if (kb == KB) {
+        kb = 0;
+        t += gridDim.x;
+      }
+      if (kb == 0)
+        idesc = sm100::idesc_f8(half_last && place(t).y == p.tiles_n - 1 ? BN / 2 : BN);
       const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1, bph = (g >> 1) & 1;
+      if ((g & 1) != b) {
+        if (!sm100::mbar_wait(&sh->full[s], ph, p.err, 73)) break;
+        if (leader) sm100::mbar_arrive(&sh->empty[s]);
+        __syncwarp();
+        continue;
+      }
       if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72) ||
           !sm100::mbar_wait(&sh->full[s], ph, p.err, 73))
         break;
@@ -348,13 +386,6 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     const int row = 32 * q + lane;
     constexpr int kCols = BN / 2;          // columns of this thread
     constexpr int kChunks = kCols / 32;
-    // first TMEM column of chunk c, and which of the two weight scales it has
-    auto col_of = [&](int c) {
-      if constexpr (EPI == kFbGlu)
-        return c < kChunks / 2 ? half * (BN / 4) + 32 * c : BN / 2 + half * (BN / 4) + 32 * (c - kChunks / 2);
-      else
-        return half * kCols + 32 * c;
-    };
     uint32_t g = 0;
     // A warp whose wait ran out goes through its remaining tiles without
     // waiting or storing: the other warps count on it at the barriers below.
@@ -364,12 +395,12 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     float a = 0.0f, w0 = 0.0f, w1 = 0.0f;
     // a tile's scales: pointers, and the values of its first K step
     auto open_tile = [&](int t) {
-      ti = fb_tile<BN, EPI>(p, sh->tile_off, t);
+      ti = fb_tile<BN, EPI>(p, tile_off, place(t));
       sa = p.sa + (ti.row0 + (row < ti.rows ? row : 0)) * KB;
       const float* se = p.sw + ti.expert * p.NB * KB;
       // a run of columns that lies past the last row of w reads the last
       // scale; its sums are not used
-      const int64_t c0 = min(ti.n0 + col_of(0), p.N - 1);
+      const int64_t c0 = min(ti.n0 + half * (EPI == kFbGlu ? BN / 4 : kCols), p.N - 1);
       const int64_t c1 = EPI == kFbGlu ? min(p.I + ti.n0 + half * (BN / 4), p.N - 1) : c0;
       sw0 = se + (c0 / kFbBlock) * KB;
       sw1 = se + (c1 / kFbBlock) * KB;
@@ -379,8 +410,15 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     };
     if ((int)blockIdx.x < total) open_tile(blockIdx.x);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      if (!alive) open_tile(t);      // (a live warp opened it in the last K step of the tile before)
       const FbTile cur = ti;
+      if (half && !has_two(cur.n0)) {      // these columns do not exist: only hand the buffers back
+        for (int kb = 0; kb < KB; ++kb, ++g) {
+          if (alive) alive = sm100::mbar_wait(&sh->acc_full[g & 1], (g >> 1) & 1, p.err, 75);
+          if (alive && lane == 0) sm100::mbar_arrive(&sh->acc_empty[g & 1]);
+        }
+        if (t + (int)gridDim.x < total) open_tile(t + gridDim.x);
+        continue;
+      }
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
@@ -391,23 +429,21 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           a = __ldg(sa + kb + 1);
           w0 = __ldg(sw0 + kb + 1);
           w1 = __ldg(sw1 + kb + 1);
-        } else if (t + (int)gridDim.x < total) {
-          open_tile(t + gridDim.x);
         }
         if (!alive || !sm100::mbar_wait(&sh->acc_full[b], bph, p.err, 74)) {
           alive = false;
           break;
         }
         sm100::tc_fence_after();
-        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * BN + half * kCols;
         // the read of a chunk of 32 columns runs under the sums of the last
         uint32_t r[2][32];
-        sm100::tmem_ld32_nowait(tq + col_of(0), r[0]);
+        sm100::tmem_ld32_nowait(tq, r[0]);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           sm100::tmem_ld_wait();
           if (c + 1 < kChunks) {
-            sm100::tmem_ld32_nowait(tq + col_of(c + 1), r[(c + 1) & 1]);
+            sm100::tmem_ld32_nowait(tq + 32 * (c + 1), r[(c + 1) & 1]);
           } else {
             sm100::tc_fence_before();
             __syncwarp();
@@ -418,11 +454,23 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), cs, acc[32 * c + i]);
         }
       }
-      if constexpr (EPI == kFbStore)
-        fb_store_half<kCols>(p, tmO, cur, base + L::kStages * L::kStage + half * (128 * kCols * 2), acc, row, half,
-                             alive);
-      else
-        fb_glu_half(p, cur, sh->amax, true, acc, row, half, alive);
+      if (t + (int)gridDim.x < total) open_tile(t + gridDim.x);   // its loads run under the stores
+      if constexpr (EPI == kFbStore) {
+        if (p.bias) {
+          const int64_t n0 = cur.n0 + half * kCols;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) acc[i] += n0 + i < p.N ? __bfloat162float(p.bias[n0 + i]) : 0.0f;
+        }
+        // the last tile's TMA stores have read this half's room
+        uint8_t* box = base + L::kStages * L::kStage + half * (128 * kCols * 2);
+        if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+        if (p.out_tma && (cur.rows == 128 || !p.grp_off)) fb_store_tile(p, tmO, cur, box, acc, row, half, alive);
+        else if (p.out_dt == AEOQ_BF16) fb_store_rows<__nv_bfloat16>(p, cur, box + q * 4096, acc, q, half, alive);
+        else fb_store_rows<float>(p, cur, box + q * 4096, acc, q, half, alive);
+      } else {
+        fb_glu_half(p, cur, sh->amax, has_two(cur.n0), acc, row, half, alive);
+      }
     }
   }
   // the stores' reads of shared memory are over before it goes away
@@ -442,10 +490,10 @@ static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbPar
   CUtensorMap ta, tw, to;
   int rc = make_tmap_bytes(&ta, a, a_rows, p.K, p.K, 128, 128, true);
   if (rc) return rc;
-  rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, EPI == kFbGlu ? BN / 2 : BN, true);
+  rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, EPI == kFbGlu ? BN / 4 : BN, true);
   if (rc) return rc;
   to = ta;
-  p.out_tma = L::kOut > 0 && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+  p.out_tma = EPI == kFbStore && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
   if (p.out_tma) {
     rc = make_tmap_bytes(&to, p.out, p.M, p.N * 2, p.ldc * 2, 128, 128, true);
     if (rc) return rc;
@@ -456,294 +504,6 @@ static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbPar
   const int ctas = (int)std::min<int64_t>(device_sm_count(), max_tiles);
   fp8_block_gemm_kernel<BN, EPI><<<ctas, kFbThreads, L::kBytes, st>>>(ta, tw, to, p);
   return check_launch("fp8_block_gemm_kernel");
-}
-
-// ---------------------------------------------------------------- CTA pairs
-// The same GEMM with two CTAs per tile (cta_group::2): 256 tokens x 256
-// columns, each CTA with 128 tokens and all columns. Against one CTA per
-// 128 x 256 tile it needs 32 KB instead of 48 KB of operands per SM and K
-// step (the step's MMAs take 512 cycles, and an SM gets about 64 bytes per
-// cycle from L2), and half of the shared-memory reads of w.
-//
-// A step's MMAs come as two groups of 128 columns with accumulators of their
-// own ("halves"): four warps per CTA scale each half, and a half's buffer is
-// free again 256 + scaling + about 380 cycles (MMAs, and the way from their
-// commit over the scaling warps back to the issuer) after its MMAs began,
-// which with two buffers each just keeps the tensor cores busy.
-//
-//   warp 0      TMA into this CTA; the bytes of both count on rank 0's barrier
-//   warps 1-2   in rank 0: MMA issuers, one per half
-//   warps 4-11  scaling and epilogue: warps 4-7 half 0, warps 8-11 half 1
-//
-// Columns of half h: store n0 + 128 h .. + 127; GLU gate n0 + 64 h .. + 63 and
-// the 64 up columns that go with them. The part of w that is half h's
-// operand in rank r: rows n0 + 128 h + 64 r (store), gate (r = 0) or up
-// (r = 1) rows n0 + 64 h (GLU). A half that lies past the last column is left
-// out.
-template <int EPI>
-struct FbPairLayout {
-  static constexpr uint32_t kA = 128 * 128, kBHalf = 64 * 128, kStage = kA + 2 * kBHalf;
-  static constexpr uint32_t kOut = EPI == kFbStore ? 128 * 256 * 2 : 0;
-  struct Ctl {
-    uint64_t full[kFbMaxStages], empty[kFbMaxStages];
-    uint64_t acc_full[2][2], acc_empty[2][2];     // [buffer][half]
-    uint32_t tmem_base;
-    float amax[2][128];
-    int tile_off[kFbMaxExperts + 1];
-  };
-  static constexpr int kStages =
-      std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl) - (int)kOut) / (int)kStage);
-  static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + kOut + sizeof(Ctl);
-};
-
-// Tiles of 256 rows: rows of this CTA's half (rank 0 the first 128).
-template <int EPI>
-__device__ __forceinline__ FbTile fb_pair_tile(const FbParams& p, const int* tile_off, int t, int rank) {
-  FbTile r;
-  const int mt = t / p.tiles_n;
-  r.n0 = (int64_t)(t - mt * p.tiles_n) * (EPI == kFbGlu ? 128 : 256);
-  int64_t end;
-  if (!p.grp_off) {
-    r.expert = 0;
-    r.row0 = (int64_t)mt * 256;
-    end = p.M;
-  } else {
-    int lo = 0, hi = p.E;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tile_off[mid] <= mt) lo = mid; else hi = mid;
-    }
-    r.expert = lo;
-    r.row0 = __ldg(p.grp_off + lo) + (mt - tile_off[lo]) * 256;
-    end = __ldg(p.grp_off + lo + 1);
-  }
-  r.row0 += 128 * rank;
-  r.rows = (int)min((int64_t)128, max((int64_t)0, end - r.row0));
-  return r;
-}
-
-template <int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFbThreads, 1)
-    fp8_block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                               const __grid_constant__ CUtensorMap tmO, const FbParams p) {
-  using L = FbPairLayout<EPI>;
-  extern __shared__ __align__(1024) uint8_t dsmem[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
-  auto* sh = reinterpret_cast<typename L::Ctl*>(base + L::kStages * L::kStage + L::kOut);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)sm100::cluster_ctarank();
-
-  if (tid == 0) {
-    for (int s = 0; s < L::kStages; ++s) {
-      sm100::mbar_init(&sh->full[s], 1);
-      sm100::mbar_init(&sh->empty[s], 2);            // a commit of each issuer
-    }
-    for (int i = 0; i < 4; ++i) {
-      sm100::mbar_init(&sh->acc_full[0][0] + i, 1);
-      sm100::mbar_init(&sh->acc_empty[0][0] + i, kFbEpiWarps);   // four warps of each CTA
-    }
-    sm100::fence_barrier_init();
-    sm100::prefetch_tmap(&tmA);
-    sm100::prefetch_tmap(&tmW);
-    if (EPI == kFbStore && p.out_tma) sm100::prefetch_tmap(&tmO);
-  }
-  if (p.grp_off)
-    for (int e = tid; e <= p.E; e += kFbThreads) sh->tile_off[e] = p.tile_off[e];
-  if (warp == 1) sm100::tmem_alloc_pair(&sh->tmem_base, 512);
-  sm100::tc_fence_before();
-  __syncthreads();
-  sm100::cluster_sync();       // the peer's barriers are ready too
-  sm100::tc_fence_after();
-  const uint32_t tmem = sh->tmem_base;
-  const int total = (p.grp_off ? sh->tile_off[p.E] : (int)p.tiles_m) * p.tiles_n;
-  const int first = (int)sm100::cluster_id_x(), step = (int)sm100::cluster_count_x();
-  const int KB = p.KB;
-  // does half 1 of the tile at column n0 exist?
-  auto two = [&](int64_t n0) { return EPI == kFbGlu ? n0 + 64 < p.I : n0 + 128 < p.N; };
-
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFbRegsLow));
-    if (warp == 0) {
-      // ---------------------------------------------------------- producer
-      const bool leader = sm100::elect_one();
-      uint32_t g = 0;
-      bool alive = true;
-      for (int t = first; t < total && alive; t += step) {
-        const FbTile ti = fb_pair_tile<EPI>(p, sh->tile_off, t, rank);
-        const int64_t w0 = ti.expert * p.N + ti.n0 + (EPI == kFbGlu ? rank * p.I : 64 * rank);
-        const bool h1 = two(ti.n0);
-        for (int kb = 0; kb < KB; ++kb, ++g) {
-          const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
-          if (!sm100::mbar_wait(&sh->empty[s], ph ^ 1, p.err, 81)) { alive = false; break; }
-          if (leader) {
-            uint8_t* st = base + s * L::kStage;
-            const uint32_t bar = sm100::dsmem_addr(&sh->full[s], 0);
-            if (rank == 0)
-              sm100::mbar_arrive_expect_tx(&sh->full[s], 2 * (L::kA + (h1 ? 2 : 1) * L::kBHalf));
-            sm100::tma_load_2d_pair(st, &tmA, kb * 128, (int32_t)ti.row0, bar);
-            sm100::tma_load_2d_pair(st + L::kA, &tmW, kb * 128, (int32_t)w0, bar);
-            if (h1)
-              sm100::tma_load_2d_pair(st + L::kA + L::kBHalf, &tmW, kb * 128,
-                                      (int32_t)(w0 + (EPI == kFbGlu ? 64 : 128)), bar);
-          }
-          __syncwarp();
-        }
-      }
-      // Every commit into this CTA has arrived before it may leave.
-      for (uint32_t i = 0; i < (uint32_t)L::kStages && alive; ++i, ++g) {
-        if (g < (uint32_t)L::kStages) continue;
-        alive = sm100::mbar_wait(&sh->empty[g % L::kStages], ((g / L::kStages) & 1) ^ 1, p.err, 82);
-      }
-    } else if (rank == 0 && warp < 3) {
-      // ------------------------------------------------------- MMA issuers
-      // One per half. A parity wait is only sound where its waiter holds back
-      // the barrier's next phase: each issuer waits for every K step and
-      // each step's stage is free once both have committed it, half 1's in
-      // tiles without a half 1 too.
-      const bool leader = sm100::elect_one();
-      constexpr uint32_t idesc = sm100::idesc_f8_pair(128);
-      const int h = warp - 1;
-      uint32_t g = 0, n = 0;           // K steps, and groups of this half, so far
-      bool alive = true;
-      for (int t = first; t < total && alive; t += step) {
-        const int mt = t / p.tiles_n;
-        const bool h1 = two((int64_t)(t - mt * p.tiles_n) * (EPI == kFbGlu ? 128 : 256));
-        for (int kb = 0; kb < KB; ++kb, ++g) {
-          const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
-          if (h && !h1) {
-            alive = sm100::mbar_wait(&sh->full[s], ph, p.err, 83);
-            if (!alive) break;
-            if (leader) sm100::tc_commit_pair(&sh->empty[s]);
-            __syncwarp();
-            continue;
-          }
-          const uint32_t b = n & 1, bph = (n >> 1) & 1;
-          ++n;
-          alive = sm100::mbar_wait_two(&sh->full[s], ph, &sh->acc_empty[b][h], bph ^ 1, p.err, 84);
-          if (!alive) break;
-          sm100::tc_fence_after();
-          if (leader) {
-            const uint32_t sa = sm100::smem_u32(base + s * L::kStage), sb = sa + L::kA + h * L::kBHalf;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              sm100::tc_mma_f8_pair(tmem + b * 256 + h * 128, sm100::sdesc_k_sw128(sa + 32 * j),
-                                    sm100::sdesc_k_sw128(sb + 32 * j), idesc, j ? 1u : 0u);
-            sm100::tc_commit_pair(&sh->acc_full[b][h]);
-            sm100::tc_commit_pair(&sh->empty[s]);
-          }
-          __syncwarp();
-        }
-      }
-    }
-  } else {
-    // ------------------------------------------------------------ epilogue
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFbRegsHigh));
-    const int q = warp & 3, half = (warp - 4) >> 2;
-    const int row = 32 * q + lane;
-    const uint32_t empty0 = sm100::dsmem_addr(&sh->acc_empty[0][half], 0);
-    uint32_t n = 0;       // groups of this half so far
-    // A warp whose wait ran out goes through its remaining tiles without
-    // waiting or storing: the other warps count on it at the barriers below.
-    bool alive = true;
-    FbTile ti{};
-    const float *sa = p.sa, *sw0 = p.sw, *sw1 = p.sw;
-    float a = 0.0f, w0 = 0.0f, w1 = 0.0f;
-    // this thread's first column (GLU: first gate column) in the tile
-    const int c_half = EPI == kFbGlu ? 64 * half : 128 * half;
-    // the next tile of which this half exists, from t on: its scales' pointers
-    // and the values of its first K step
-    auto open_tile = [&](int t) {
-      for (; t < total; t += step) {
-        ti = fb_pair_tile<EPI>(p, sh->tile_off, t, rank);
-        if (half == 0 || two(ti.n0)) break;
-      }
-      if (t >= total) return total;
-      sa = p.sa + (ti.rows > 0 ? ti.row0 + (row < ti.rows ? row : 0) : 0) * KB;
-      const float* se = p.sw + ti.expert * p.NB * KB;
-      sw0 = se + ((ti.n0 + c_half) / kFbBlock) * KB;
-      sw1 = EPI == kFbGlu ? se + ((p.I + ti.n0 + c_half) / kFbBlock) * KB : sw0;
-      a = __ldg(sa);
-      w0 = __ldg(sw0);
-      w1 = __ldg(sw1);
-      return t;
-    };
-    int t = open_tile(first);
-    while (t < total) {
-      const FbTile cur = ti;
-      int t_next = total;
-      float acc[128];
-#pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-      for (int kb = 0; kb < KB; ++kb, ++n) {
-        const uint32_t b = n & 1, bph = (n >> 1) & 1;
-        const float c0 = a * w0, c1 = a * w1;
-        if (kb + 1 < KB) {
-          a = __ldg(sa + kb + 1);
-          w0 = __ldg(sw0 + kb + 1);
-          if (EPI == kFbGlu) w1 = __ldg(sw1 + kb + 1);
-        } else {
-          t_next = open_tile(t + step);
-        }
-        if (alive) alive = sm100::mbar_wait(&sh->acc_full[b][half], bph, p.err, 85);
-        if (!alive) continue;
-        sm100::tc_fence_after();
-        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * 256 + half * 128;
-        // the read of a chunk of 32 columns runs under the sums of the last
-        uint32_t r[2][32];
-        sm100::tmem_ld32_nowait(tq, r[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sm100::tmem_ld_wait();
-          if (c + 1 < 4) {
-            sm100::tmem_ld32_nowait(tq + 32 * (c + 1), r[(c + 1) & 1]);
-          } else {
-            sm100::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) sm100::mbar_arrive_cluster(empty0 + b * 2 * sizeof(uint64_t));
-          }
-          const float cs = (EPI == kFbGlu && c >= 2) ? c1 : c0;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), cs, acc[32 * c + i]);
-        }
-      }
-      if constexpr (EPI == kFbStore)
-        fb_store_half<128>(p, tmO, cur, base + L::kStages * L::kStage + half * 32768, acc, row, half, alive);
-      else
-        fb_glu_half(p, cur, sh->amax, two(cur.n0), acc, row, half, alive);
-      t = t_next;
-    }
-    if (EPI == kFbStore) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  }
-  sm100::tc_fence_before();
-  __syncthreads();
-  sm100::cluster_sync();
-  if (warp == 1) {
-    sm100::tc_fence_after();
-    sm100::tmem_dealloc_pair(tmem, 512);
-  }
-}
-
-template <int EPI>
-static int launch_gemm_pair(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbParams p, int64_t max_tiles,
-                            cudaStream_t st) {
-  using L = FbPairLayout<EPI>;
-  CUtensorMap ta, tw, to;
-  int rc = make_tmap_bytes(&ta, a, a_rows, p.K, p.K, 128, 128, true);
-  if (rc) return rc;
-  rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, 64, true);
-  if (rc) return rc;
-  to = ta;
-  p.out_tma = EPI == kFbStore && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
-  if (p.out_tma) {
-    rc = make_tmap_bytes(&to, p.out, p.M, p.N * 2, p.ldc * 2, 128, 128, true);
-    if (rc) return rc;
-  }
-  AEOQ_REQUIRE(max_tiles <= 0x7FFFFFFF, AEOQ_ERR_INVALID, "fp8_block_gemm: too many tiles");
-  rc = func_smem_attr((const void*)fp8_block_gemm_pair_kernel<EPI>, L::kBytes, -1, "fp8_block_gemm_pair");
-  if (rc) return rc;
-  const int pairs = (int)std::min<int64_t>(device_sm_count() / 2, max_tiles);
-  fp8_block_gemm_pair_kernel<EPI><<<2 * pairs, kFbThreads, L::kBytes, st>>>(ta, tw, to, p);
-  return check_launch("fp8_block_gemm_pair_kernel");
 }
 
 static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_t* w, const float* sw, int64_t N,
@@ -762,13 +522,12 @@ static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_
   p.ldc = ldc;
   p.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
   p.err = err;
-  // Pairs once their 256 x 256 tiles fill the SMs; below that tiles of 128 x
-  // 128, of which there are more.
-  p.tiles_m = (M + 255) / 256;
-  p.tiles_n = (int)((N + 255) / 256);
-  if (2 * p.tiles_m * p.tiles_n >= device_sm_count())
-    return launch_gemm_pair<kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
+  // Tiles of 256 columns once they fill the SMs; below that 128, of which
+  // there are more.
   p.tiles_m = (M + 127) / 128;
+  p.tiles_n = (int)((N + 255) / 256);
+  if (p.tiles_m * p.tiles_n >= device_sm_count())
+    return launch_gemm<256, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
   p.tiles_n = (int)((N + 127) / 128);
   return launch_gemm<128, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
 }
@@ -776,10 +535,10 @@ static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_
 // ---------------------------------------------------------------- experts
 // Pairs (token, slot) sorted by expert: a counting sort in one CTA.
 //   grp_off[e]   first row of expert e        (E + 1 values)
-//   tile_off[e]  tiles of `tile` rows before expert e (E + 1 values)
+//   tile_off[e]  128-row tiles before expert e (E + 1 values)
 //   row_tok[r]   token of sorted row r;  pair_row[i]  row of pair i, or -1
 __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_dt, int64_t n_pairs, int k, int E,
-                                                       int tile, int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
+                                                       int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
   __shared__ int cnt[kFbMaxExperts], fill[kFbMaxExperts];
   __shared__ int s_row[32], s_tile[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -790,7 +549,7 @@ __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_
     if (e >= 0 && e < E) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
-  const int c = cnt[t], d = (c + tile - 1) / tile;      // experts past E count 0
+  const int c = cnt[t], d = (c + 127) / 128;      // experts past E count 0
   int r = c, q = d;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -963,17 +722,14 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   auto ints = [&](size_t o) { return reinterpret_cast<int*>(ws + o); };
   auto floats = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
   const int64_t P = T * k;
-  // CTA pairs (256-row tiles) where the experts have rows for them.
-  const bool pair = P >= 128 * E;
-  const int tile = pair ? 256 : 128;
-  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, tile, ints(l.grp_off), ints(l.tile_off),
+  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, ints(l.grp_off), ints(l.tile_off),
                                      ints(l.row_tok), ints(l.pair_row));
   int rc = check_launch("fb_sort_kernel");
   if (rc) return rc;
   rc = fb_quantize_rows(hidden, AEOQ_BF16, P, H, H, ints(l.row_tok), ints(l.grp_off) + E, ws + l.xq, H,
                         floats(l.xs), st);
   if (rc) return rc;
-  const int64_t max_tiles = std::min<int64_t>(P, (P + tile - 1) / tile + E);
+  const int64_t max_tiles = std::min<int64_t>(P, (P + 127) / 128 + E);
   FbParams p{};
   p.M = P;
   p.N = 2 * I;
@@ -993,8 +749,7 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   p.hs = floats(l.hs);
   p.hs_ld = fb_blocks(I);
   p.err = err_word;
-  rc = pair ? launch_gemm_pair<kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st)
-            : launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
+  rc = launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
   if (rc) return rc;
   FbParams d{};
   d.M = P;
@@ -1012,8 +767,7 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   d.out_dt = AEOQ_BF16;
   d.ldc = H;
   d.err = err_word;
-  rc = pair ? launch_gemm_pair<kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st)
-            : launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
+  rc = launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
   if (rc) return rc;
   const int64_t pieces = T * (H / 8);
   const unsigned blocks = (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)device_sm_count() * 16);

@@ -98,84 +98,6 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ uint32_t cluster_id_x() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_count_x() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-  return r;
-}
-// Arrival on a barrier of any CTA of the cluster (an address from dsmem_addr).
-// It orders no memory of its own at cluster scope (that would cost a fence
-// per arrival): for hand-overs of TMEM, which the tcgen05 fences order.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-// Both of two barriers. A try_wait
-// that succeeds at once still costs its thread about 100 cycles; issued
-// together, two of them cost little more than one.
-__device__ __forceinline__ bool mbar_wait_two(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* err,
-                                                      int code) {
-  for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 q, [%3], %4;\n\t"
-        "and.pred p, p, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(a)), "r"(pa), "r"(smem_u32(b)), "r"(pb)
-        : "memory");
-    if (ok) return true;
-  }
-  if (err) atomicCAS(err, 0, code);
-  return false;
-}
-
-// ---------------------------------------------------------------- CTA pairs
-// tcgen05 with cta_group::2: two CTAs of a cluster (an even rank and the next)
-// work on one MMA. Each holds 128 rows of A and of D, and half of B's rows.
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// 2D tile load into this CTA whose bytes count on the barrier at `bar_addr`, in
-// this CTA or its peer (from dsmem_addr).
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int32_t x, int32_t y,
-                                                 uint32_t bar_addr) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_addr)
-      : "memory");
-}
-// Arrival on the barrier at this offset in both CTAs once the MMAs issued so
-// far by this thread are done.
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_taddr, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_taddr),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y,
                                             uint64_t* bar) {
@@ -310,11 +232,6 @@ __host__ __device__ constexpr uint32_t idesc_nvf4(uint32_t n) {
 // Instruction descriptor: kind::f8f6f4, E4M3 x E4M3 -> F32, K-major, M = 128.
 __host__ __device__ constexpr uint32_t idesc_f8(uint32_t n) {
   return (1u << 4) | (0u << 7) | (0u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
-// The same with M = 256 over a CTA pair.
-__host__ __device__ constexpr uint32_t idesc_f8_pair(uint32_t n) {
-  return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
 
 }  // namespace sm100
