@@ -28,36 +28,40 @@ __global__ void __launch_bounds__(32 * kFbRowWarps) fb_rows_kernel(
   const int b_end = min(nb, ((int)blockIdx.y + 1) * chunk);
   constexpr int U = 4;   // blocks in flight per half-warp
   for (int b0 = (int)blockIdx.y * chunk; b0 < b_end; b0 += 2 * U) {
-    float v[U][8];
+    FbEight<DT> v[U];
+    uint32_t key[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int b = b0 + 2 * u + half;
       const int64_t k0 = (int64_t)b * kFbBlock + 8 * sub;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
       if (b < b_end && k0 < K) {
-        if (VEC) {
-          fb_load8<DT>(xr + k0, v[u]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (k0 + i < K) v[u][i] = In<DT>::load(xr + k0 + i);
-        }
+        if (VEC) v[u].load(xr + k0);
+        else v[u].load_some(xr + k0, K - k0);
+      } else {
+        v[u].zero();
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      key[u] = v[u].key();
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) key[u] = FbEight<DT>::key_max(key[u], __shfl_xor_sync(0xFFFFFFFFu, key[u], o));
+    }
+    // the two divisions of block u in lanes u, u + 4, .. of its half-warp alone
+    uint32_t mine = key[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) mine = (sub & 3) == u ? key[u] : mine;
+    const float2 s = fb_scales(FbEight<DT>::key_value(mine));
+    if (sub < U && b0 + 2 * sub + half < b_end) sr[b0 + 2 * sub + half] = s.y;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       const int b = b0 + 2 * u + half;
       const int64_t k0 = (int64_t)b * kFbBlock + 8 * sub;
-      uint32_t key = fb_key8(v[u]);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
-      const float2 s = fb_scales(fb_key_value(key));
-      if (b >= b_end) continue;
-      if (sub == 0) sr[b] = s.y;
-      const uint2 c = fb_codes8(v[u], s.x);
+      const float inv = __shfl_sync(0xFFFFFFFFu, s.x, (lane & 16) | u);
+      if (b >= b_end || k0 >= K) continue;
+      const uint2 c = fb_codes8(v[u], inv);
       if (VEC) {
-        if (k0 < K) *reinterpret_cast<uint2*>(qr + k0) = c;
+        *reinterpret_cast<uint2*>(qr + k0) = c;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -78,31 +82,27 @@ __global__ void __launch_bounds__(256) fb_weights_kernel(const typename In<DT>::
   const int64_t k0 = kb * kFbBlock + 8 * (threadIdx.x & 15);
   const int64_t n0 = nb * kFbBlock + (threadIdx.x >> 4);
   const typename In<DT>::T* xe = x + e * N * K;
-  float v[8][8];
-  uint32_t key = 0;
+  FbEight<DT> v[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int64_t n = n0 + 16 * r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
     if (n < N && k0 < K) {
-      if (VEC) {
-        fb_load8<DT>(xe + n * K + k0, v[r]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k0 + i < K) v[r][i] = In<DT>::load(xe + n * K + k0 + i);
-      }
+      if (VEC) v[r].load(xe + n * K + k0);
+      else v[r].load_some(xe + n * K + k0, K - k0);
+    } else {
+      v[r].zero();
     }
   }
+  uint32_t key = v[0].key();
 #pragma unroll
-  for (int r = 0; r < 8; ++r) key = max(key, fb_key8(v[r]));
-  key = __reduce_max_sync(0xFFFFFFFFu, key);
+  for (int r = 1; r < 8; ++r) key = FbEight<DT>::key_max(key, v[r].key());
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) key = FbEight<DT>::key_max(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = key;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) key = max(key, part[i]);
-  const float2 s = fb_scales(fb_key_value(key));
+  for (int i = 0; i < 8; ++i) key = FbEight<DT>::key_max(key, part[i]);
+  const float2 s = fb_scales(FbEight<DT>::key_value(key));
   if (threadIdx.x == 0) scale[(e * gridDim.y + nb) * gridDim.x + kb] = s.y;
   uint8_t* qe = q + e * N * K;
 #pragma unroll

@@ -36,33 +36,63 @@ __device__ __forceinline__ uint32_t fb_codes4(float a, float b, float c, float d
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-// Eight consecutive input values as floats.
-template <int DT>
-__device__ __forceinline__ void fb_load8(const typename In<DT>::T* p, float (&v)[8]) {
-  if constexpr (DT == AEOQ_F32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const typename In<DT>::T* e = reinterpret_cast<const typename In<DT>::T*>(&u);
+// Eight consecutive input values, as they came (16 bytes, 32 for f32: the
+// registers that a value costs while its block's maximum is not known yet).
+template <int DT> struct FbEight {
+  using T = typename In<DT>::T;
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load_some(const T* p, int64_t n) {
+    __align__(16) T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = In<DT>::to_f(e[i]);
+    for (int i = 0; i < 8; ++i) {
+      v[i] = T(0.0f);
+      if (i < n) v[i] = p[i];
+    }
+    u = *reinterpret_cast<const uint4*>(v);
   }
-}
-
-// Largest magnitude as an ordered bit pattern: NaN above infinity.
-__device__ __forceinline__ uint32_t fb_key8(const float (&v)[8]) {
-  uint32_t k = 0;
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  // Largest magnitude as an ordered key: two 16-bit patterns side by side, NaN
+  // above infinity.
+  __device__ __forceinline__ uint32_t key() const {
+    constexpr uint32_t m = 0x7FFF7FFFu;
+    return __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+  }
+  static __device__ __forceinline__ uint32_t key_max(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ float key_value(uint32_t k) { return In<DT>::key_to_f(max(k >> 16, k & 0xFFFFu)); }
+  __device__ __forceinline__ float at(int i) const { return In<DT>::to_f(reinterpret_cast<const T*>(&u)[i]); }
+};
+template <> struct FbEight<AEOQ_F32> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void load_some(const float* p, int64_t n) {
+    float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) k = max(k, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return k;
-}
-__device__ __forceinline__ float fb_key_value(uint32_t k) { return __uint_as_float(k); }
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+    a = make_float4(v[0], v[1], v[2], v[3]);
+    b = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ float at(int i) const {
+    return i < 4 ? (i < 2 ? (i ? a.y : a.x) : (i == 2 ? a.z : a.w)) : (i < 6 ? (i == 4 ? b.x : b.y) : (i == 6 ? b.z : b.w));
+  }
+  __device__ __forceinline__ uint32_t key() const {
+    uint32_t k = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k = max(k, __float_as_uint(at(i)) & 0x7FFFFFFFu);
+    return k;
+  }
+  static __device__ __forceinline__ uint32_t key_max(uint32_t x, uint32_t y) { return max(x, y); }
+  static __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k); }
+};
 
-__device__ __forceinline__ uint2 fb_codes8(const float (&v)[8], float inv) {
-  return make_uint2(fb_codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                    fb_codes4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+template <int DT>
+__device__ __forceinline__ uint2 fb_codes8(const FbEight<DT>& v, float inv) {
+  return make_uint2(fb_codes4(v.at(0) * inv, v.at(1) * inv, v.at(2) * inv, v.at(3) * inv),
+                    fb_codes4(v.at(4) * inv, v.at(5) * inv, v.at(6) * inv, v.at(7) * inv));
 }
 
 // Rows [0, rows) of x (or x[idx[r]], r < *n_rows) quantized per 128 values; their

@@ -591,10 +591,10 @@ __global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __
       const int r = __ldg(pair_row + t * k + j);
       if (r < 0) continue;
       const float w = __ldg(weights + t * k + j);
-      float v[8];
-      fb_load8<AEOQ_BF16>(y + r * H + 8 * c, v);
+      FbEight<AEOQ_BF16> v;
+      v.load(y + r * H + 8 * c);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) s[x] = fmaf(w, v[x], s[x]);
+      for (int x = 0; x < 8; ++x) s[x] = fmaf(w, v.at(x), s[x]);
     }
     __align__(16) __nv_bfloat162 o[4];
 #pragma unroll
