@@ -95,6 +95,29 @@ __device__ __forceinline__ uint2 fb_codes8(const FbEight<DT>& v, float inv) {
                     fb_codes4(v.at(4) * inv, v.at(5) * inv, v.at(6) * inv, v.at(7) * inv));
 }
 
+enum FbActivation : int { kFbGeluTanh = 0, kFbSilu = 1 };
+
+// gelu(x, tanh form) = x * sigmoid(2 z), z = sqrt(2/pi) (x + 0.044715 x^3),
+// since 1 + tanh(z) = 2 sigmoid(2 z); silu(x) = x * sigmoid(x). Written so,
+// neither cancels for negative x. __expf's relative error grows with its
+// argument (about 2^-22 + |arg| 2^-24); where |arg| is large the result is 0
+// or x to within f32.
+__device__ __forceinline__ float fb_act(int act, float x) {
+  const float a = act == kFbSilu ? x : 1.5957691216057308f * (x + 0.044715f * (x * x * x));
+  return __fdividef(x, 1.0f + __expf(-a));
+}
+
+// Few rows of a: the weights are streamed through mma.sync (fp8_block_skinny.cu).
+constexpr int kFbSkinnyRows = 64;        // linear: rows at most
+bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K);
+int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uint8_t* w, const float* sw, int64_t N,
+                     int64_t K, const void* bias, void* out, int out_dt, int64_t ldc, uint8_t* q, float* qs,
+                     cudaStream_t st);
+bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I);
+int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt, const float* weights, int64_t k,
+                      const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,
+                      int64_t I, int act, float* h, void* out, cudaStream_t st);
+
 // Rows [0, rows) of x (or x[idx[r]], r < *n_rows) quantized per 128 values; their
 // scales (rows, ceil(K / 128)).
 int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, const int* idx,

@@ -46,7 +46,6 @@ constexpr int kFbMaxStages = 8;
 constexpr int kFbMaxExperts = 1024;
 
 enum FbEpilogue : int { kFbStore = 0, kFbGlu = 1 };
-enum FbActivation : int { kFbGeluTanh = 0, kFbSilu = 1 };
 
 struct FbParams {
   int64_t M;              // rows of a (dense), or the most there can be (grouped)
@@ -127,16 +126,6 @@ __device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off
   r.row0 = g0 + (mt - tile_off[lo]) * 128;
   r.rows = min(128, g1 - (int)r.row0);
   return r;
-}
-
-// gelu(x, tanh form) = x * sigmoid(2 z), z = sqrt(2/pi) (x + 0.044715 x^3),
-// since 1 + tanh(z) = 2 sigmoid(2 z); silu(x) = x * sigmoid(x). Written so,
-// neither cancels for negative x. __expf's relative error grows with its
-// argument (about 2^-22 + |arg| 2^-24); where |arg| is large the result is 0
-// or x to within f32.
-__device__ __forceinline__ float fb_act(int act, float x) {
-  const float a = act == kFbSilu ? x : 1.5957691216057308f * (x + 0.044715f * (x * x * x));
-  return __fdividef(x, 1.0f + __expf(-a));
 }
 
 // ---------------------------------------------------------------- epilogues
@@ -603,9 +592,9 @@ __global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __
   }
 }
 
-// Workspace of the grouped forward.
+// Workspace: of the grouped forward, or of that for few tokens (h alone).
 struct FbExpertsWs {
-  size_t grp_off, tile_off, row_tok, pair_row, xq, xs, hq, hs, y, bytes;
+  size_t grp_off = 0, tile_off = 0, row_tok = 0, pair_row = 0, xq = 0, xs = 0, hq = 0, hs = 0, y = 0, h = 0, bytes = 0;
   FbExpertsWs(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
     size_t o = 0;
     const int64_t P = T * k;
@@ -614,6 +603,11 @@ struct FbExpertsWs {
       o += (size_t)((n + 255) / 256 * 256);
       return at;
     };
+    if (fb_experts_skinny_takes(T, k, E, H, I)) {
+      h = take(4 * P * I);
+      bytes = o;
+      return;
+    }
     grp_off = take(4 * (E + 1));
     tile_off = take(4 * (E + 1));
     row_tok = take(4 * P);
@@ -650,6 +644,9 @@ extern "C" int aeoq_fp8_block_gemm(const uint8_t* a, const float* sa, int64_t M,
   AEOQ_REQUIRE(a && sa && w && sw && out, AEOQ_ERR_INVALID, "fp8_block_gemm: null pointer");
   AEOQ_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0, AEOQ_ERR_INVALID,
                "fp8_block_gemm: operands must be 16-byte aligned");
+  if (fb_linear_skinny_takes(M, N, K))
+    return fb_linear_skinny(nullptr, AEOQ_BF16, K, M, w, sw, N, K, bias, out, out_dtype, ldc, const_cast<uint8_t*>(a),
+                            const_cast<float*>(sa), (cudaStream_t)stream);
   return gemm_dense(a, sa, M, w, sw, N, K, bias, out, out_dtype, ldc, err_word, (cudaStream_t)stream);
 }
 
@@ -678,6 +675,8 @@ extern "C" int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int6
   cudaStream_t st = (cudaStream_t)stream;
   uint8_t* q = reinterpret_cast<uint8_t*>(workspace);
   float* s = reinterpret_cast<float*>(q + linear_scales_at(M, K));
+  if (fb_linear_skinny_takes(M, N, K))
+    return fb_linear_skinny(x, dtype, ldx, M, w, sw, N, K, bias, out, out_dtype, ldc, q, s, st);
   rc = fb_quantize_rows(x, dtype, M, K, ldx, nullptr, nullptr, q, K, s, st);
   if (rc) return rc;
   return gemm_dense(q, s, M, w, sw, N, K, bias, out, out_dtype, ldc, err_word, st);
@@ -722,6 +721,9 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   auto ints = [&](size_t o) { return reinterpret_cast<int*>(ws + o); };
   auto floats = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
   const int64_t P = T * k;
+  if (fb_experts_skinny_takes(T, k, E, H, I))
+    return fb_experts_skinny(hidden, T, top_k_index, idx_dtype, top_k_weights, k, gate_up, gate_up_scale, down,
+                             down_scale, E, H, I, activation, floats(l.h), out, st);
   fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, ints(l.grp_off), ints(l.tile_off),
                                      ints(l.row_tok), ints(l.pair_row));
   int rc = check_launch("fb_sort_kernel");
