@@ -400,7 +400,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     if ((int)blockIdx.x < total) open_tile(blockIdx.x);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const FbTile cur = ti;
-      if (half && !has_two(cur.n0)) {      // these columns do not exist: only hand the buffers back
+      const bool both = has_two(cur.n0);
+      if (half && !both) {      // these columns do not exist: only hand the buffers back
         for (int kb = 0; kb < KB; ++kb, ++g) {
           if (alive) alive = sm100::mbar_wait(&sh->acc_full[g & 1], (g >> 1) & 1, p.err, 75);
           if (alive && lane == 0) sm100::mbar_arrive(&sh->acc_empty[g & 1]);
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         else if (p.out_dt == AEOQ_BF16) fb_store_rows<__nv_bfloat16>(p, cur, box + q * 4096, acc, q, half, alive);
         else fb_store_rows<float>(p, cur, box + q * 4096, acc, q, half, alive);
       } else {
-        fb_glu_half(p, cur, sh->amax, has_two(cur.n0), acc, row, half, alive);
+        fb_glu_half(p, cur, sh->amax, both, acc, row, half, alive);
       }
     }
   }
@@ -495,6 +496,238 @@ static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbPar
   return check_launch("fp8_block_gemm_kernel");
 }
 
+// ---------------------------------------------------------------- few rows per expert
+// The grouped GEMMs for experts with few tokens: bound by the weights' bytes,
+// if nothing else takes longer. With tokens on the MMA's 128 rows the scaling
+// of 256 columns does (16 tokens over 128 experts: 78 + 49 us for 505 MB), so
+// here the weights are the MMA's rows and up to 32 tokens its columns: a
+// thread owns one output feature and 16 tokens, a K step costs it 32 sums.
+//
+// Tile: 256 rows of w as two MMAs of 128 (GLU: 128 gate rows and the 128 up
+// rows that go with them; store: 256 consecutive ones) times 32 tokens.
+//   warp 0 TMA, warp 1 MMA and TMEM, warps 4-11 scaling and epilogue: four
+//   warps with tokens 0-15, four with tokens 16-31
+struct FbFewLayout {
+  static constexpr int kTok = 32;
+  static constexpr uint32_t kA = 256 * 128, kB = kTok * 128, kStage = kA + kB;
+  struct Ctl {
+    uint64_t full[kFbMaxStages], empty[kFbMaxStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    uint32_t amax[2][4][16];             // GLU: [token half][lane quadrant][token]
+    int tile_off[kFbMaxExperts + 1];
+  };
+  static constexpr int kStages =
+      std::min<int>(kFbMaxStages, (227 * 1024 - 1024 - (int)sizeof(Ctl)) / (int)kStage);
+  static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + sizeof(Ctl);
+  static constexpr uint32_t kTmemCols = 128;   // 2 buffers x 2 MMAs x 32 tokens
+};
+
+template <int EPI>
+__global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __grid_constant__ CUtensorMap tmW,
+                                                                     const __grid_constant__ CUtensorMap tmB,
+                                                                     const FbParams p) {
+  using L = FbFewLayout;
+  extern __shared__ __align__(1024) uint8_t dsmem[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
+  auto* sh = reinterpret_cast<L::Ctl*>(base + L::kStages * L::kStage);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      sm100::mbar_init(&sh->full[s], 1);
+      sm100::mbar_init(&sh->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      sm100::mbar_init(&sh->acc_full[b], 1);
+      sm100::mbar_init(&sh->acc_empty[b], kFbEpiWarps);
+    }
+    sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tmW);
+    sm100::prefetch_tmap(&tmB);
+  }
+  for (int e = tid; e <= p.E; e += kFbThreads) sh->tile_off[e] = p.tile_off[e];
+  if (warp == 1) sm100::tmem_alloc(&sh->tmem_base, L::kTmemCols);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const int total = sh->tile_off[p.E] * p.tiles_n, KB = p.KB;
+  constexpr int kWide = EPI == kFbGlu ? 128 : 256;      // output columns of a tile
+  auto tile = [&](int t) {
+    FbTile r;
+    const int ct = t / p.tiles_n;
+    r.n0 = (int64_t)(t - ct * p.tiles_n) * kWide;
+    int lo = 0, hi = p.E;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sh->tile_off[mid] <= ct) lo = mid; else hi = mid;
+    }
+    r.expert = lo;
+    const int g0 = __ldg(p.grp_off + lo), g1 = __ldg(p.grp_off + lo + 1);
+    r.row0 = g0 + (ct - sh->tile_off[lo]) * L::kTok;
+    r.rows = min(L::kTok, g1 - (int)r.row0);
+    return r;
+  };
+
+  if (warp == 0) {
+    const bool leader = sm100::elect_one();
+    uint32_t g = 0;
+    bool alive = true;
+    for (int t = blockIdx.x; t < total && alive; t += gridDim.x) {
+      const FbTile ti = tile(t);
+      const int w0 = (int)(ti.expert * p.N + ti.n0);
+      // boxes of 64 rows of w: those that hold an output column
+      const int left = (int)((EPI == kFbGlu ? p.I : p.N) - ti.n0), boxes = min(kWide / 64, (left + 63) / 64);
+      for (int kb = 0; kb < KB; ++kb, ++g) {
+        const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
+        if (!sm100::mbar_wait(&sh->empty[s], ph ^ 1, p.err, 81)) { alive = false; break; }
+        if (leader) {
+          uint8_t* st = base + s * L::kStage;
+          sm100::mbar_arrive_expect_tx(&sh->full[s], L::kB + (uint32_t)boxes * (EPI == kFbGlu ? 2 : 1) * 8192);
+          for (int i = 0; i < boxes; ++i) {
+            sm100::tma_load_2d(st + i * 8192, &tmW, kb * 128, w0 + 64 * i, &sh->full[s]);
+            if (EPI == kFbGlu)
+              sm100::tma_load_2d(st + 16384 + i * 8192, &tmW, kb * 128, w0 + (int)p.I + 64 * i, &sh->full[s]);
+          }
+          sm100::tma_load_2d(st + L::kA, &tmB, kb * 128, (int)ti.row0, &sh->full[s]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = sm100::elect_one();
+    constexpr uint32_t idesc = sm100::idesc_f8(L::kTok);
+    const int mine = (int)blockIdx.x < total ? (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+    const uint32_t steps = (uint32_t)mine * KB;
+    for (uint32_t g = 0; g < steps; ++g) {
+      const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1, b = g & 1, bph = (g >> 1) & 1;
+      if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 82) ||
+          !sm100::mbar_wait(&sh->full[s], ph, p.err, 83))
+        break;
+      sm100::tc_fence_after();
+      if (leader) {
+        const uint32_t sa = sm100::smem_u32(base + s * L::kStage), sb = sa + L::kA;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sm100::tc_mma_f8(tmem + b * 64 + m * 32, sm100::sdesc_k_sw128(sa + m * 16384 + 32 * j),
+                             sm100::sdesc_k_sw128(sb + 32 * j), idesc, j ? 1u : 0u);
+        sm100::tc_commit(&sh->empty[s]);
+        sm100::tc_commit(&sh->acc_full[b]);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    const int q = warp & 3, half = (warp - 4) >> 2, f = 32 * q + lane;      // f: row of w in each MMA
+    uint32_t g = 0;
+    bool alive = true;      // as in the kernel above
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const FbTile ti = tile(t);
+      const int tok0 = 16 * half, n_tok = min(16, ti.rows - tok0);
+      if (n_tok <= 0) {
+        for (int kb = 0; kb < KB; ++kb, ++g) {
+          if (alive) alive = sm100::mbar_wait(&sh->acc_full[g & 1], (g >> 1) & 1, p.err, 84);
+          if (alive && lane == 0) sm100::mbar_arrive(&sh->acc_empty[g & 1]);
+        }
+        continue;
+      }
+      // lane j's token scale; the two MMAs' weight scales (rows past the last
+      // one take its scale, their sums are not used)
+      const float* sa = p.sa + (ti.row0 + tok0 + min(lane & 15, n_tok - 1)) * KB;
+      const float* se = p.sw + ti.expert * p.NB * KB;
+      const int64_t c0 = min(ti.n0 + f, p.N - 1), c1 = min((EPI == kFbGlu ? p.I : 128) + ti.n0 + f, p.N - 1);
+      const float *sw0 = se + (c0 / kFbBlock) * KB, *sw1 = se + (c1 / kFbBlock) * KB;
+      float acc[2][16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[0][j] = acc[1][j] = 0.0f;
+      float a = __ldg(sa), w0 = __ldg(sw0), w1 = __ldg(sw1);
+      for (int kb = 0; kb < KB; ++kb, ++g) {
+        const uint32_t b = g & 1, bph = (g >> 1) & 1;
+        const float a_now = a, w0_now = w0, w1_now = w1;
+        if (kb + 1 < KB) {
+          a = __ldg(sa + kb + 1);
+          w0 = __ldg(sw0 + kb + 1);
+          w1 = __ldg(sw1 + kb + 1);
+        }
+        if (alive) alive = sm100::mbar_wait(&sh->acc_full[b], bph, p.err, 85);
+        if (!alive) continue;
+        sm100::tc_fence_after();
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * 64 + tok0;
+        float r0[16], r1[16];
+        sm100::tmem_ld16(tq, r0);
+        sm100::tmem_ld16(tq + 32, r1);
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sh->acc_empty[b]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float c = __shfl_sync(0xFFFFFFFFu, a_now, j);
+          acc[0][j] = fmaf(r0[j], c * w0_now, acc[0][j]);
+          acc[1][j] = fmaf(r1[j], c * w1_now, acc[1][j]);
+        }
+      }
+      if constexpr (EPI == kFbStore) {
+        // 32 lanes store 64 consecutive bytes of a token's row
+        __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + (ti.row0 + tok0) * p.ldc + ti.n0 + f;
+        if (!alive) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (j >= n_tok) break;
+          if (ti.n0 + f < p.N) d[j * p.ldc] = __float2bfloat16_rn(acc[0][j]);
+          if (ti.n0 + 128 + f < p.N) d[j * p.ldc + 128] = __float2bfloat16_rn(acc[1][j]);
+        }
+      } else {
+        // the block of 128 features of a token is this tile's 128 lanes
+        const bool in = ti.n0 + f < p.I;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          acc[0][j] = in ? fb_act(p.act, acc[0][j]) * acc[1][j] : 0.0f;
+          const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(acc[0][j]) & 0x7FFFFFFFu);
+          if (lane == j) sh->amax[half][q][j] = k;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+        uint32_t k = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k = max(k, sh->amax[half][i][lane & 15]);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+        const float2 s = fb_scales(__uint_as_float(k));      // of token lane & 15
+        if (!alive) continue;
+        if (q == 0 && lane < n_tok) p.hs[(ti.row0 + tok0 + lane) * p.hs_ld + ti.n0 / kFbBlock] = s.y;
+        uint8_t* d = p.hq + (ti.row0 + tok0) * p.hq_ld + ti.n0 + f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float inv = __shfl_sync(0xFFFFFFFFu, s.x, j);
+          if (j < n_tok && in) d[j * p.hq_ld] = (uint8_t)fb_codes4(acc[0][j] * inv, 0.0f, 0.0f, 0.0f);
+        }
+      }
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+template <int EPI>
+static int launch_few(const uint8_t* a, int64_t a_rows, const uint8_t* w, const FbParams& p, int64_t max_tiles,
+                      cudaStream_t st) {
+  using L = FbFewLayout;
+  CUtensorMap tw, tb;
+  int rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, 64, true);
+  if (rc) return rc;
+  rc = make_tmap_bytes(&tb, a, a_rows, p.K, p.K, 128, L::kTok, true);
+  if (rc) return rc;
+  AEOQ_REQUIRE(max_tiles <= 0x7FFFFFFF, AEOQ_ERR_INVALID, "fp8_block_few: too many tiles");
+  rc = func_smem_attr((const void*)fp8_block_few_kernel<EPI>, L::kBytes, -1, "fp8_block_few");
+  if (rc) return rc;
+  const int ctas = (int)std::min<int64_t>(device_sm_count(), max_tiles);
+  fp8_block_few_kernel<EPI><<<ctas, kFbThreads, L::kBytes, st>>>(tw, tb, p);
+  return check_launch("fp8_block_few_kernel");
+}
+
 static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_t* w, const float* sw, int64_t N,
                       int64_t K, const void* bias, void* out, int out_dt, int64_t ldc, int* err, cudaStream_t st) {
   FbParams p{};
@@ -524,10 +757,10 @@ static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_
 // ---------------------------------------------------------------- experts
 // Pairs (token, slot) sorted by expert: a counting sort in one CTA.
 //   grp_off[e]   first row of expert e        (E + 1 values)
-//   tile_off[e]  128-row tiles before expert e (E + 1 values)
+//   tile_off[e]  tiles of `tile` rows before expert e (E + 1 values)
 //   row_tok[r]   token of sorted row r;  pair_row[i]  row of pair i, or -1
 __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_dt, int64_t n_pairs, int k, int E,
-                                                       int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
+                                                       int tile, int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
   __shared__ int cnt[kFbMaxExperts], fill[kFbMaxExperts];
   __shared__ int s_row[32], s_tile[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -538,7 +771,7 @@ __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_
     if (e >= 0 && e < E) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
-  const int c = cnt[t], d = (c + 127) / 128;      // experts past E count 0
+  const int c = cnt[t], d = (c + tile - 1) / tile;      // experts past E count 0
   int r = c, q = d;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -724,14 +957,19 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   if (fb_experts_skinny_takes(T, k, E, H, I))
     return fb_experts_skinny(hidden, T, top_k_index, idx_dtype, top_k_weights, k, gate_up, gate_up_scale, down,
                              down_scale, E, H, I, activation, floats(l.h), out, st);
-  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, ints(l.grp_off), ints(l.tile_off),
+  // Weights on the MMA's rows up to 40 rows per expert: at 128 experts, top-8,
+  // H = 2816, I = 704 (cold L2) 64 tokens take 170 us that way and 228 the
+  // other, 512 tokens (32 rows) 205 and 244, 1024 tokens (64 rows) 328 and 260.
+  const bool few = P <= 40 * E;
+  const int tile = few ? FbFewLayout::kTok : 128;
+  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, tile, ints(l.grp_off), ints(l.tile_off),
                                      ints(l.row_tok), ints(l.pair_row));
   int rc = check_launch("fb_sort_kernel");
   if (rc) return rc;
   rc = fb_quantize_rows(hidden, AEOQ_BF16, P, H, H, ints(l.row_tok), ints(l.grp_off) + E, ws + l.xq, H,
                         floats(l.xs), st);
   if (rc) return rc;
-  const int64_t max_tiles = std::min<int64_t>(P, (P + 127) / 128 + E);
+  const int64_t max_tiles = std::min<int64_t>(P, (P + tile - 1) / tile + E);
   FbParams p{};
   p.M = P;
   p.N = 2 * I;
@@ -751,7 +989,8 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   p.hs = floats(l.hs);
   p.hs_ld = fb_blocks(I);
   p.err = err_word;
-  rc = launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
+  rc = few ? launch_few<kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st)
+           : launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
   if (rc) return rc;
   FbParams d{};
   d.M = P;
@@ -769,7 +1008,8 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   d.out_dt = AEOQ_BF16;
   d.ldc = H;
   d.err = err_word;
-  rc = launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
+  rc = few ? launch_few<kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st)
+           : launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
   if (rc) return rc;
   const int64_t pieces = T * (H / 8);
   const unsigned blocks = (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)device_sm_count() * 16);

@@ -57,21 +57,14 @@ struct SkWeights {
 
 // This lane's 32 values of column g in one block, quantized: codes and the
 // block's scale. v: the lane's piece (null: zeros); n: values of it that exist
-// (a multiple of 16). CG: the values come from a kernel that may still have
-// been running when this one started, and are read past L1.
-template <int DT, bool CG>
+// (a multiple of 16).
+template <int DT>
 __device__ __forceinline__ void sk_quantize(const typename In<DT>::T* v, int64_t n, uint32_t (&c)[8], float& scale) {
   FbEight<DT> e[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (v && 8 * i < n) {
-      if constexpr (CG) {
-        static_assert(!CG || DT == AEOQ_F32, "");
-        e[i].a = __ldcg(reinterpret_cast<const float4*>(v + 8 * i));
-        e[i].b = __ldcg(reinterpret_cast<const float4*>(v + 8 * i) + 1);
-      } else {
-        e[i].load(v + 8 * i);
-      }
+      e[i].load(v + 8 * i);
     } else {
       e[i].zero();
     }
@@ -153,7 +146,7 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
         float xs = 0.0f, d[4];
         if constexpr (QUANT) {
           const auto* x = reinterpret_cast<const typename In<DT>::T*>(p.x);
-          sk_quantize<DT, false>(m < p.M ? x + m * p.ldx + k0 : nullptr, p.K - k0, c, xs);
+          sk_quantize<DT>(m < p.M ? x + m * p.ldx + k0 : nullptr, p.K - k0, c, xs);
         } else {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -230,8 +223,6 @@ int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uin
 }
 
 // ----------------------------------------------------------------- experts
-constexpr int kSkMaxPairs = 512;
-
 struct SkExperts {
   const __nv_bfloat16* hidden;
   const void* ids; int ids_dt;
@@ -244,74 +235,109 @@ struct SkExperts {
   __nv_bfloat16* out;       // (T, H)
 };
 
-// h = act(gate x) * up x for the pairs (token, slot) of one expert. CTA (x, y):
-// features 8 x .. 8 x + 7 (their gate rows are the MMA's rows 0-7, their up rows
-// 8-15) of the expert of pair y, if y is the first pair with it: an expert's
-// weights are read once for all its tokens, eight at a time.
-__global__ void __launch_bounds__(kSkThreads) sk_gate_up_kernel(const SkExperts p) {
-  __shared__ float part[kSkWarps][32][4];
-  __shared__ int list[kSkMaxPairs];
-  __shared__ int n_list;
+// One warp's codes of a row of one block, four values per lane: written to
+// `codes` (128 bytes) in shared memory, the scale returned to every lane.
+__device__ __forceinline__ float sk_quantize_warp(const float (&v)[4], uint8_t* codes) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) key = max(key, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  key = __reduce_max_sync(0xFFFFFFFFu, key);
+  const float2 s = fb_scales(__uint_as_float(key));
+  reinterpret_cast<uint32_t*>(codes)[lane] = fb_codes4(v[0] * s.x, v[1] * s.x, v[2] * s.x, v[3] * s.x);
+  return s.y;
+}
+
+// A lane's piece of a row's codes in shared memory, for every column alike.
+__device__ __forceinline__ void sk_codes(const uint8_t* codes, uint32_t (&c)[8]) {
+  const uint4* q = reinterpret_cast<const uint4*>(codes + 32 * (threadIdx.x & 3));
+  const uint4 a = q[0], b = q[1];
+  c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+  c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
+}
+
+// h = act(gate x) * up x of one pair (token, slot). CTA (x, y): features 8 x ..
+// 8 x + 7 (their gate rows are the MMA's rows 0-7, their up rows 8-15) of pair
+// y. Four warps and few registers, so that the 88 x 8 CTAs of one token at I =
+// 704 are all on the 148 SMs at once: a CTA's time is that of a chain of
+// memory latencies, and with two CTAs of eight warps per SM it was paid in
+// three waves (17.6 us).
+constexpr int kSkGuWarps = 4;
+__global__ void __launch_bounds__(32 * kSkGuWarps, 5) sk_gate_up_kernel(const SkExperts p) {
+  __shared__ float part[kSkGuWarps][16];
+  __shared__ __align__(16) uint8_t codes[kSkGuWarps][kSkAhead][128];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int P = p.T * p.k, y = blockIdx.y;
+  const int y = blockIdx.y, f0 = blockIdx.x * 8;
   const int64_t e = load_index(p.ids, p.ids_dt, y);
-  if (threadIdx.x == 0) n_list = 0;
-  bool seen = e < 0 || e >= p.E;
-  for (int i = threadIdx.x; i < y; i += kSkThreads) seen |= load_index(p.ids, p.ids_dt, i) == e;
-  if (__syncthreads_or(seen)) return;
-  for (int i = y + threadIdx.x; i < P; i += kSkThreads)
-    if (load_index(p.ids, p.ids_dt, i) == e) list[atomicAdd(&n_list, 1)] = i;
-  __syncthreads();
-  const int n = n_list, f0 = blockIdx.x * 8;
-  const int64_t rows = e * 2 * p.I;
-  const uint8_t* w0 = p.gu + (rows + f0 + g) * p.H;
+  const __nv_bfloat16* x = p.hidden + (int64_t)(y / p.k) * p.H + 4 * lane;
+  if (e < 0 || e >= p.E) return;
+  const uint8_t* w0 = p.gu + (e * 2 * p.I + f0 + g) * p.H;
   const uint8_t* w1 = w0 + (int64_t)p.I * p.H;
   const float* s0 = p.gus + (e * p.NBgu + f0 / kFbBlock) * p.KBH;
   const float* s1 = p.gus + (e * p.NBgu + (p.I + f0) / kFbBlock) * p.KBH;
-  for (int b = 0; b < n; b += 8) {
-    const int pair = b + g < n ? list[b + g] : -1;
-    const __nv_bfloat16* x = pair >= 0 ? p.hidden + (int64_t)(pair / p.k) * p.H + 32 * t : nullptr;
-    float acc[4] = {};
-    for (int kb0 = warp; kb0 < p.KBH; kb0 += kSkWarps * kSkAhead) {
-      SkWeights w[kSkAhead];
-      float sg[kSkAhead], su[kSkAhead];
+  float acc0 = 0.0f, acc1 = 0.0f;
+  for (int kb0 = warp; kb0 < p.KBH; kb0 += kSkGuWarps * kSkAhead) {
+    SkWeights w[kSkAhead];
+    float sg[kSkAhead], su[kSkAhead], xs[kSkAhead];
+    uint2 xv[kSkAhead];
 #pragma unroll
-      for (int u = 0; u < kSkAhead; ++u) {
-        const int kb = kb0 + u * kSkWarps;
-        w[u].load(w0, w1, kb * kFbBlock + 32 * t, kb < p.KBH ? p.H : 0);
-        sg[u] = kb < p.KBH ? __ldg(s0 + kb) : 0.0f;
-        su[u] = kb < p.KBH ? __ldg(s1 + kb) : 0.0f;
-      }
-#pragma unroll
-      for (int u = 0; u < kSkAhead; ++u) {
-        const int kb = kb0 + u * kSkWarps;
-        if (kb >= p.KBH) break;
-        uint32_t c[8];
-        float xs, d[4];
-        sk_quantize<AEOQ_BF16, false>(x ? x + kb * kFbBlock : nullptr, p.H - kb * kFbBlock - 32 * t, c, xs);
-        w[u].dot(d, c);
-        sk_add(acc, d, xs, sg[u], su[u]);
-      }
+    for (int u = 0; u < kSkAhead; ++u) {
+      const int kb = kb0 + u * kSkGuWarps;
+      const bool in = kb < p.KBH;
+      xv[u] = in && kb * kFbBlock + 4 * lane < p.H ? __ldg(reinterpret_cast<const uint2*>(x + kb * kFbBlock))
+                                                    : make_uint2(0u, 0u);
+      w[u].load(w0, w1, kb * kFbBlock + 32 * t, in ? p.H : 0);
+      sg[u] = in ? __ldg(s0 + kb) : 0.0f;
+      su[u] = in ? __ldg(s1 + kb) : 0.0f;
     }
-    if (b) __syncthreads();
-    *reinterpret_cast<float4*>(part[warp][lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    __syncthreads();
-    const int row = threadIdx.x & 7, col = threadIdx.x >> 3;
-    if (threadIdx.x < 64 && b + col < n)
-      p.h[(int64_t)list[b + col] * p.I + f0 + row] = fb_act(p.act, sk_sum(part, row, col)) * sk_sum(part, row + 8, col);
+#pragma unroll
+    for (int u = 0; u < kSkAhead; ++u) {
+      const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&xv[u]);
+      const float v[4] = {__bfloat162float(b[0]), __bfloat162float(b[1]), __bfloat162float(b[2]),
+                          __bfloat162float(b[3])};
+      xs[u] = sk_quantize_warp(v, codes[warp][u]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kSkAhead; ++u) {
+      if (kb0 + u * kSkGuWarps >= p.KBH) break;
+      uint32_t c[8];
+      float d[4];
+      sk_codes(codes[warp][u], c);
+      w[u].dot(d, c);
+      acc0 = fmaf(d[0], xs[u] * sg[u], acc0);
+      acc1 = fmaf(d[2], xs[u] * su[u], acc1);
+    }
+    __syncwarp();
+  }
+  if (t == 0) {                  // every column is the same
+    part[warp][g] = acc0;
+    part[warp][g + 8] = acc1;
+  }
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    float gate = 0.0f, up = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSkGuWarps; ++w) {
+      gate += part[w][threadIdx.x];
+      up += part[w][threadIdx.x + 8];
+    }
+    p.h[(int64_t)y * p.I + f0 + threadIdx.x] = fb_act(p.act, gate) * up;
   }
 }
 
 // out[t] = sum over slots of weight * down h. CTA (x, y): output columns 16 x ..
-// + 15 of token y; warp w takes the slots w, w + 8, .. (one token: the MMA's
-// other seven columns are zeros). The weights of a warp's first slot are
-// requested before the kernel that writes h is known to be done.
-__global__ void __launch_bounds__(kSkThreads) sk_down_kernel(const SkExperts p) {
+// + 15 of token y; warp w takes the slots w, w + 8, ... The weights of a warp's
+// first slot are requested before the kernel that writes h is known to be
+// done; h is quantized by each CTA for itself, a block per warp and step.
+__global__ void __launch_bounds__(kSkThreads, 2) sk_down_kernel(const SkExperts p) {
+  constexpr int U = 6;                   // K blocks in flight: all of them up to I = 768
   __shared__ float part[kSkWarps][16];
+  __shared__ __align__(16) uint8_t codes[kSkWarps][U][128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16, y = blockIdx.y;
-  float total0 = 0.0f, total1 = 0.0f;      // rows g and g + 8 (valid in lanes t = 0)
+  float total0 = 0.0f, total1 = 0.0f;      // rows g and g + 8
   bool waited = false;
   for (int j = warp; j < p.k; j += kSkWarps) {
     const int pair = y * p.k + j;
@@ -321,35 +347,48 @@ __global__ void __launch_bounds__(kSkThreads) sk_down_kernel(const SkExperts p) 
     const uint8_t* w0 = n0 + g < p.H ? p.dw + (e * p.H + n0 + g) * p.I : nullptr;
     const uint8_t* w1 = n0 + 8 + g < p.H ? p.dw + (e * p.H + n0 + 8 + g) * p.I : nullptr;
     const float* sd = p.dws + (e * p.NBd + n0 / kFbBlock) * p.KBI;
-    const float* h = g == 0 ? p.h + (int64_t)pair * p.I + 32 * t : nullptr;
-    float acc[4] = {};
-    constexpr int U = 6;                   // K blocks in flight: all of them up to I = 768
+    const float* h = p.h + (int64_t)pair * p.I + 4 * lane;
+    float acc0 = 0.0f, acc1 = 0.0f;
     for (int kb0 = 0; kb0 < p.KBI; kb0 += U) {
       SkWeights w[U];
-      float s[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kb = kb0 + u;
-        w[u].load(w0, w1, kb * kFbBlock + 32 * t, kb < p.KBI ? p.I : 0);
-        s[u] = kb < p.KBI ? __ldg(sd + kb) : 0.0f;
-      }
+      for (int u = 0; u < U; ++u) w[u].load(w0, w1, (kb0 + u) * kFbBlock + 32 * t, kb0 + u < p.KBI ? p.I : 0);
+      // lane u keeps the weight scale of block u, then times h's
+      float s = lane < U && kb0 + lane < p.KBI ? __ldg(sd + kb0 + lane) : 0.0f;
       if (!waited) {
         pdl_wait();
         waited = true;
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kb = kb0 + u;
-        if (kb >= p.KBI) break;
-        uint32_t c[8];
-        float hs, d[4];
-        sk_quantize<AEOQ_F32, true>(h ? h + kb * kFbBlock : nullptr, p.I - kb * kFbBlock - 32 * t, c, hs);
-        w[u].dot(d, c);
-        sk_add(acc, d, hs, s[u], s[u]);
+      for (int u0 = 0; u0 < U; u0 += 3) {
+        float4 v[3];
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+          const int k = (kb0 + u0 + u) * kFbBlock;
+          v[u] = k + 4 * lane < p.I ? __ldcg(reinterpret_cast<const float4*>(h + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+          const float f[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          const float hs = sk_quantize_warp(f, codes[warp][u0 + u]);
+          if (lane == u0 + u) s *= hs;
+        }
       }
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t c[8];
+        float d[4];
+        sk_codes(codes[warp][u], c);
+        w[u].dot(d, c);
+        const float f = __shfl_sync(0xFFFFFFFFu, s, u);
+        acc0 = fmaf(d[0], f, acc0);
+        acc1 = fmaf(d[2], f, acc1);
+      }
+      __syncwarp();
     }
-    total0 = fmaf(weight, acc[0], total0);
-    total1 = fmaf(weight, acc[2], total1);
+    total0 = fmaf(weight, acc0, total0);
+    total1 = fmaf(weight, acc1, total1);
   }
   if (!waited) pdl_wait();
   if (t == 0) {
@@ -365,9 +404,11 @@ __global__ void __launch_bounds__(kSkThreads) sk_down_kernel(const SkExperts p) 
   }
 }
 
-bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
-  return T * k <= kSkMaxPairs && T * k <= 4 * E && T <= 64;
-}
+// Every pair reads its expert's weights here, the grouped GEMMs read each
+// expert's once but need five launches: at 128 experts, top-8, H = 2816, I =
+// 704 one token takes 23 us (cold L2), 4 tokens 51 against 70, 8 tokens (64
+// pairs) 86 against 90, 16 tokens 158 against 125.
+bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) { return T * k <= 64; }
 
 int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt, const float* weights, int64_t k,
                       const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,
@@ -393,7 +434,7 @@ int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt
   p.act = act;
   p.h = h;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  sk_gate_up_kernel<<<dim3((unsigned)(I / 8), (unsigned)(T * k)), kSkThreads, 0, st>>>(p);
+  sk_gate_up_kernel<<<dim3((unsigned)(I / 8), (unsigned)(T * k)), 32 * kSkGuWarps, 0, st>>>(p);
   int rc = check_launch("sk_gate_up_kernel");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
