@@ -72,12 +72,9 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 __device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    v = u > v ? u : v;
-  }
-  return v;
+  const uint32_t hi = __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return ((uint64_t)hi << 32) | lo;
 }
 
 template <int DT>
@@ -142,7 +139,28 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
   if (p.n_group > 1) {
     const int S = p.E / p.n_group;
     double worth = -INFINITY;
-    for (int g = 0; g < p.n_group; ++g) {
+    const int lpg = S / PER;
+    const bool whole = S % PER == 0 && (lpg & (lpg - 1)) == 0;
+    if (whole) {
+      uint64_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (key[i] > a) { b = a; a = key[i]; }
+        else if (key[i] > b) b = key[i];
+      }
+      for (int o = 1; o < lpg; o <<= 1) {
+        const uint64_t c = __shfl_xor_sync(0xFFFFFFFFu, a, o), d = __shfl_xor_sync(0xFFFFFFFFu, b, o);
+        const uint64_t low = a < c ? a : c;
+        b = b > d ? b : d;
+        b = b > low ? b : low;
+        a = a > c ? a : c;
+      }
+      double v = order_val64(a);
+      if (p.top2 && b > kNegInfKey64) v += order_val64(b);
+      worth = __shfl_sync(0xFFFFFFFFu, v, lane * lpg);
+      if (lane >= p.n_group) worth = -INFINITY;
+    }
+    for (int g = 0; g < p.n_group && !whole; ++g) {
       uint64_t a = 0, b = 0;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -310,24 +328,45 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
   if (p.n_group > 1) {
     const int S = p.E / p.n_group;
     float worth = -INFINITY;
-    for (int g = 0; g < p.n_group; ++g) {
+    const int lpg = S / PER;         // lanes per group
+    if (S % PER == 0 && (lpg & (lpg - 1)) == 0) {
+      // all groups at once: each lane's two largest, then those of the lanes
+      // of its group
       uint32_t a = 0, b = 0;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = lane * PER + i;
-        if (e >= g * S && e < (g + 1) * S) {
-          b = max(b, min(a, key[i]));
-          a = max(a, key[i]);
+        b = max(b, min(a, key[i]));
+        a = max(a, key[i]);
+      }
+      for (int o = 1; o < lpg; o <<= 1) {
+        const uint32_t c = __shfl_xor_sync(0xFFFFFFFFu, a, o), d = __shfl_xor_sync(0xFFFFFFFFu, b, o);
+        b = max(max(b, d), min(a, c));
+        a = max(a, c);
+      }
+      float v = order_val(a);
+      if (p.top2 && b > kNegInfKey) v += order_val(b);
+      worth = __shfl_sync(0xFFFFFFFFu, v, lane * lpg);     // lane g holds group g's
+      if (lane >= p.n_group) worth = -INFINITY;
+    } else {
+      for (int g = 0; g < p.n_group; ++g) {
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int e = lane * PER + i;
+          if (e >= g * S && e < (g + 1) * S) {
+            b = max(b, min(a, key[i]));
+            a = max(a, key[i]);
+          }
         }
+        const uint32_t ga = __reduce_max_sync(0xFFFFFFFFu, a);
+        float v = order_val(ga);
+        if (p.top2) {
+          const int who = __ffs(__ballot_sync(0xFFFFFFFFu, a == ga)) - 1;
+          const uint32_t gb = __reduce_max_sync(0xFFFFFFFFu, lane == who ? b : a);
+          if (gb > kNegInfKey) v += order_val(gb);
+        }
+        if (lane == g) worth = v;
       }
-      const uint32_t ga = __reduce_max_sync(0xFFFFFFFFu, a);
-      float v = order_val(ga);
-      if (p.top2) {
-        const int who = __ffs(__ballot_sync(0xFFFFFFFFu, a == ga)) - 1;
-        const uint32_t gb = __reduce_max_sync(0xFFFFFFFFu, lane == who ? b : a);
-        if (gb > kNegInfKey) v += order_val(gb);
-      }
-      if (lane == g) worth = v;
     }
     bool near = false;
     const uint32_t keep = keep_groups<float>(worth, p.n_group, p.topk_group, 2.0f * tol, near);
@@ -398,6 +437,142 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
   }
 }
 
+// ---------------------------------------------------------------- many rows
+// One thread per row, for 16-bit logits that alone decide (no bias, no
+// groups) and k <= 8. A logit and its index make one 32-bit key that orders
+// as they do, so a comparison of two candidates is one max and one min: eight
+// keys at a time are sorted (19 of them) and merged into the best eight so
+// far (8 + 12), 35 instructions per row and warp lane at 128 experts where
+// the warp above takes some 800. The rows are staged through shared memory,
+// read with whole lines.
+constexpr int kRouteRowThreads = 128;
+constexpr int kRouteRowsFrom = 4096;     // rows: see below
+
+__device__ __forceinline__ void key_pair(uint32_t& a, uint32_t& b) {
+  const uint32_t t = max(a, b);
+  b = min(a, b);
+  a = t;
+}
+__device__ __forceinline__ void sort8(uint32_t (&v)[8]) {      // descending
+  key_pair(v[0], v[1]); key_pair(v[2], v[3]); key_pair(v[4], v[5]); key_pair(v[6], v[7]);
+  key_pair(v[0], v[2]); key_pair(v[1], v[3]); key_pair(v[4], v[6]); key_pair(v[5], v[7]);
+  key_pair(v[1], v[2]); key_pair(v[5], v[6]); key_pair(v[0], v[4]); key_pair(v[3], v[7]);
+  key_pair(v[1], v[5]); key_pair(v[2], v[6]);
+  key_pair(v[1], v[4]); key_pair(v[3], v[6]);
+  key_pair(v[2], v[4]); key_pair(v[3], v[5]);
+  key_pair(v[3], v[4]);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kRouteRowThreads) route_rows_kernel(const RouteParams p) {
+  using Tp = typename In<DT>::T;
+  extern __shared__ __align__(16) uint8_t rows[];
+  const int64_t row0 = blockIdx.x * (int64_t)kRouteRowThreads;
+  const int n = (int)min((int64_t)kRouteRowThreads, p.T - row0);
+  const int chunks = p.E / 8, pitch = 2 * p.E + 16;       // 16 bytes more: 8 rows, 8 different bank groups
+  for (int i = threadIdx.x; i < n * chunks; i += kRouteRowThreads) {
+    const int r = i / chunks, c = i - r * chunks;
+    *reinterpret_cast<uint4*>(rows + r * pitch + 16 * c) =
+        __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const Tp*>(p.logits) + (row0 + r) * p.ld) + c);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= n) return;
+  const uint8_t* mine = rows + threadIdx.x * pitch;
+  constexpr uint32_t kInf = DT == AEOQ_BF16 ? 0x7F80u : 0x7C00u;
+  uint32_t best[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+  uint32_t most = 0;      // largest magnitude pattern: NaN above infinity
+  for (int c = 0; c < chunks; ++c) {
+    const uint4 u = *reinterpret_cast<const uint4*>(mine + 16 * c);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t b = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+      most = max(most, b & 0x7FFFu);
+      b = b == 0x8000u ? 0u : b;                                  // -0 and +0 are equal
+      b = (b & 0x8000u) ? b ^ 0xFFFFu : b | 0x8000u;
+      v[i] = (b << 16) | (0xFFFFu - (uint32_t)(8 * c + i));         // equal logits: the lower index first
+    }
+    sort8(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) best[i] = max(best[i], v[7 - i]);
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(i & d)) key_pair(best[i], best[i + d]);
+  }
+  const int64_t row = row0 + threadIdx.x;
+  float* wo = p.w + row * p.k;
+  int64_t* io = p.ids + row * p.k;
+  const auto logit = [&](uint32_t key) {
+    const uint32_t b = key >> 16;
+    return In<DT>::key_to_f((b & 0x8000u) ? b & 0x7FFFu : b ^ 0xFFFFu);
+  };
+  const float top = logit(best[0]);
+  if (most > kInf || (!p.sigmoid && top == INFINITY)) {
+    for (int j = 0; j < p.k; ++j) {
+      wo[j] = __int_as_float(0x7FC00000);
+      io[j] = j;
+    }
+    return;
+  }
+  float s[8], sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float l = logit(best[j]);
+    s[j] = 0.0f;
+    if (j < p.k && l > -INFINITY) s[j] = p.sigmoid ? __fdividef(1.0f, 1.0f + expf(-l)) : expf(l - top);
+    sum += s[j];
+  }
+  if (p.sigmoid && top > -INFINITY && sum < 1e-30f) {      // f32 has lost them
+    double d[8], t = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float l = logit(best[j]);
+      d[j] = j < p.k && l > -INFINITY ? 1.0 / (1.0 + exp(-(double)l)) : 0.0;
+      t += d[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = (float)(p.renorm ? (t > 0.0 ? d[j] / t : 0.0) : d[j]);
+    sum = 1.0f;
+  } else if (p.renorm) {
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] *= inv;
+  } else if (!p.sigmoid && top > -INFINITY) {
+    float t = 0.0f;
+    for (int c = 0; c < chunks; ++c) {
+      const uint4 u = *reinterpret_cast<const uint4*>(mine + 16 * c);
+      const Tp* e = reinterpret_cast<const Tp*>(&u);
+      float part = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part += expf(In<DT>::to_f(e[i]) - top);
+      t += part;
+    }
+    const float inv = 1.0f / t;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] *= inv;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= p.k) break;
+    const bool none = logit(best[j]) == -INFINITY;
+    wo[j] = none ? 0.0f : s[j] * p.scale;
+    io[j] = none ? p.E : (int64_t)(0xFFFFu - (best[j] & 0xFFFFu));
+  }
+}
+
+template <int DT>
+static int launch_route_rows(const RouteParams& p, cudaStream_t st) {
+  const size_t bytes = (size_t)kRouteRowThreads * (2 * p.E + 16);
+  const int rc = func_smem_attr((const void*)route_rows_kernel<DT>, bytes, -1, "route_rows");
+  if (rc) return rc;
+  const unsigned blocks = (unsigned)((p.T + kRouteRowThreads - 1) / kRouteRowThreads);
+  route_rows_kernel<DT><<<blocks, kRouteRowThreads, bytes, st>>>(p);
+  return check_launch("route_rows_kernel");
+}
+
 template <int PER, int DT>
 static int launch_route(const RouteParams& p, cudaStream_t st) {
   const unsigned blocks = (unsigned)((p.T + kRouteWarps - 1) / kRouteWarps);
@@ -415,6 +590,12 @@ static int dispatch_route(RouteParams p, cudaStream_t st) {
   const int bytes = per * (int)sizeof(typename In<DT>::T), width = std::min(bytes, 16);
   p.vec = p.E % per == 0 && (uintptr_t)p.logits % width == 0 &&
           (p.ld * (int64_t)sizeof(typename In<DT>::T)) % width == 0;
+  if constexpr (DT != AEOQ_F32) {
+    const bool logits_alone = !p.bias && p.n_group == 1;
+    if (logits_alone && p.k <= 8 && p.E >= 8 && p.E <= 512 && p.E % 8 == 0 && (uintptr_t)p.logits % 16 == 0 &&
+        (p.ld * 2) % 16 == 0 && p.T >= kRouteRowsFrom)
+      return launch_route_rows<DT>(p, st);
+  }
   switch (per) {
     case 1: return launch_route<1, DT>(p, st);
     case 2: return launch_route<2, DT>(p, st);

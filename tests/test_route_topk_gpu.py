@@ -73,6 +73,45 @@ def test_many_rows_with_bias():
         assert torch.equal(ids, want[:, :8])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k", [(4096, 128, 8), (5003, 256, 3), (4100, 8, 8), (4097, 512, 1), (4099, 136, 5),
+                                   (4096, 520, 4), (4098, 130, 8)])
+def test_many_16_bit_rows(dtype, T, E, k):
+    """The row counts at which one thread takes a row: ties, masks, NaN and
+    infinite rows among them."""
+    from aeo_quant_b200.gpu.routing import route_topk
+    inf = float("inf")
+    l = (torch.randn(T, E, generator=gen(E)) * 2).to(dtype)
+    l[torch.rand(T, E, generator=gen(E + 1)) < 0.05] = -inf
+    l[7] = -inf
+    l[8, 2:] = -inf
+    l[9] = 0.0
+    l[10] = -0.0
+    l[11, ::2] = -0.0
+    l[12, E // 2] = float("nan")
+    l[13, E - 1] = inf
+    l[14] = -300.0
+    l[15, 3:] = torch.finfo(dtype).min
+    for score in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            w, ids = route_topk(l.cuda(), k, score=score, renormalize=renorm, scale=2.0)
+            x = l.double().numpy()
+            bad = np.isnan(x).any(1) | (np.isposinf(x).any(1) if score == "softmax" else False)
+            order = np.argsort(-np.where(np.isnan(x), -inf, x), 1, kind="stable")[:, :k]
+            v = np.take_along_axis(x, order, 1)
+            with np.errstate(all="ignore"):
+                top = np.where(np.isneginf(x).all(1), 0.0, x.max(1))[:, None]
+                s = np.exp(v - top) / np.exp(x - top).sum(1, keepdims=True) if score == "softmax" else 1 / (1 + np.exp(-v))
+                s = np.where(np.isneginf(v), 0.0, s)
+                if renorm:
+                    s = np.where(s.sum(1, keepdims=True) > 0, s / s.sum(1, keepdims=True), 0.0)
+            want = np.where(bad[:, None], np.arange(k), np.where(np.isneginf(v), E, order))
+            got, w = ids.cpu().numpy(), w.cpu().numpy().astype(np.float64)
+            assert np.array_equal(got, want)
+            assert np.isnan(w[bad]).all() and not np.isnan(w[~bad]).any()
+            assert np.all(np.abs(w - 2 * s)[~bad] <= TOL * 2 * s[~bad] + 1e-37)
+
+
 def test_ties_go_to_the_lower_index():
     l = torch.zeros(4, 128).cuda()
     _, ids = check(l, 8)
