@@ -186,14 +186,40 @@ class _Here:
 _HERE = _Here()
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is current: a kernel launches on the
+def on_device(index: int):
+    """Context in which device ``index`` is current: a kernel launches on the
     current device, whichever device its pointers and stream belong to."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# The current stream's handle without a Stream object around it (0.1 instead of
+# 2.3 us, of some 12 that a one-token call takes the host).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of device ``index``."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(index).cuda_stream
+    return _raw_stream(index)
+
+
+def cuda_index(first: torch.Tensor, *rest) -> int:
+    """Index of the device that all tensors are on (``None`` among them is
+    skipped); raises where one is on the CPU, on another device, or the
+    device is not a B200."""
+    index = first.get_device()
+    if index not in _SM100_DEVICES:
+        require_cuda(first)
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            require_cuda(t)
+            raise ValueError(f"tensors are on different devices: {first.device} and {t.device}")
+    return index
 
 
 def ptr(t) -> int | None:
@@ -213,13 +239,16 @@ def err_word(device: torch.device) -> torch.Tensor:
     return t
 
 
-def err_ptr(device: torch.device):
-    """Address of the error word, or None (kernels then record nothing) when
-    it does not exist yet and a graph is being captured: made there, it
-    would live in that graph's memory."""
-    if device.index not in _ERR_WORDS and torch.cuda.is_current_stream_capturing():
-        return None
-    return err_word(device).data_ptr()
+def err_ptr(index: int):
+    """Address of device ``index``'s error word, or None (kernels then record
+    nothing) when it does not exist yet and a graph is being captured: made
+    there, it would live in that graph's memory."""
+    t = _ERR_WORDS.get(index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        t = err_word(torch.device("cuda", index))
+    return t.data_ptr()
 
 
 # Weight scale atoms are derived once per weight tensor and cached here,

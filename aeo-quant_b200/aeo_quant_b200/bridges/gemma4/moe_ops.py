@@ -390,42 +390,42 @@ def fp8_block_experts(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_s
     I = two_i // 2
     T = hidden.shape[0]
     blocks = lambda n: -(-n // 128)  # noqa: E731
-    if hidden.shape[1] != H or tuple(dw.shape) != (E, H, I) or two_i % 2:
+    if hidden.shape[1] != H or dw.shape != (E, H, I) or two_i % 2:
         raise ValueError(f"hidden {tuple(hidden.shape)}, gate_up {tuple(gu.shape)} and down {tuple(dw.shape)} "
                          "do not fit together")
     for name, t, s, want in (("gate_up", gu, gu_scale, (E, blocks(two_i), blocks(H))),
                              ("down", dw, dw_scale, (E, blocks(H), blocks(I)))):
-        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        if t.dtype != torch.float8_e4m3fn and t.dtype != torch.uint8:
             raise ValueError(f"{name} must be float8_e4m3fn, got {t.dtype}")
-        if tuple(s.shape) != want or s.dtype != torch.float32:
+        if s.shape != want or s.dtype != torch.float32:
             raise ValueError(f"{name} scales must be float32 of shape {want}, got {s.dtype} {tuple(s.shape)}")
         if not t.is_contiguous() or not s.is_contiguous():
             raise ValueError(f"{name} weights and scales must be contiguous")
     if top_k_index.ndim != 2 or top_k_index.shape[0] != T or top_k_index.shape != top_k_weights.shape:
         raise ValueError(f"top_k_index {tuple(top_k_index.shape)} and top_k_weights {tuple(top_k_weights.shape)} "
                          f"must both be ({T}, k)")
-    if top_k_index.dtype not in (torch.int32, torch.int64):
+    if top_k_index.dtype != torch.int64 and top_k_index.dtype != torch.int32:
         raise ValueError(f"top_k_index must be int32 or int64, got {top_k_index.dtype}")
     if not top_k_weights.dtype.is_floating_point:
         raise ValueError(f"top_k_weights must be floating point, got {top_k_weights.dtype}")
-    A.require_cuda(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale)
-    dev = hidden.device
-    for t in (top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale):
-        if t.device != dev:
-            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
+    dev = A.cuda_index(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_scale)
     lib = A.load()
     k = top_k_index.shape[1]
     with A.on_device(dev):
-        hidden = hidden.contiguous()
+        if not hidden.is_contiguous():
+            hidden = hidden.contiguous()
         if hidden.data_ptr() % 16:
             hidden = hidden.clone()
         ids = top_k_index.contiguous()
-        w = top_k_weights.detach().to(torch.float32).contiguous()
-        out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+        w = top_k_weights
+        if w.dtype != torch.float32:
+            w = w.detach().to(torch.float32)
+        w = w.contiguous()
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=hidden.device)
         n = lib.aeoq_moe_fp8_block_workspace_size(T, k, E, H, I)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = torch.empty(n, dtype=torch.uint8, device=hidden.device)
         A.check(lib.aeoq_moe_fp8_block_forward(
-            hidden.data_ptr(), T, ids.data_ptr(), A.dtype_code(ids.dtype), w.data_ptr(), k, gu.data_ptr(),
-            gu_scale.data_ptr(), dw.data_ptr(), dw_scale.data_ptr(), E, H, I, _ACTIVATIONS[activation],
-            out.data_ptr(), ws.data_ptr(), n, A.err_ptr(dev), A.stream_ptr(dev)))
+            hidden.data_ptr(), T, ids.data_ptr(), A.I64 if ids.dtype == torch.int64 else A.I32, w.data_ptr(), k,
+            gu.data_ptr(), gu_scale.data_ptr(), dw.data_ptr(), dw_scale.data_ptr(), E, H, I, _ACTIVATIONS[activation],
+            out.data_ptr(), ws.data_ptr(), n, A.err_ptr(dev), A.raw_stream(dev)))
     return out

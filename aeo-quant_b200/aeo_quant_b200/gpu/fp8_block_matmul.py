@@ -31,7 +31,7 @@ def _check_weight(w_fp8: torch.Tensor, w_scale: torch.Tensor) -> tuple[int, int]
         raise ValueError(f"w_fp8 must be float8_e4m3fn, got {w_fp8.dtype}")
     N, K = w_fp8.shape
     want = (-(-N // FP8_BLOCK), -(-K // FP8_BLOCK))
-    if tuple(w_scale.shape) != want or w_scale.dtype != torch.float32:
+    if w_scale.shape != want or w_scale.dtype != torch.float32:
         raise ValueError(f"w_scale must be float32 of shape {want} (one per {FP8_BLOCK} x {FP8_BLOCK} block), "
                          f"got {w_scale.dtype} {tuple(w_scale.shape)}")
     return N, K
@@ -43,12 +43,6 @@ def _check_out(out_dtype: torch.dtype, bias, N: int) -> int:
     if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.bfloat16):
         raise ValueError(f"bias must be bfloat16 of shape ({N},), got {bias.dtype} {tuple(bias.shape)}")
     return _OUT_DT[out_dtype]
-
-
-def _same_device(first: torch.Tensor, *rest) -> None:
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors are on different devices: {first.device} and {t.device}")
 
 
 def fp8_block_linear(x: torch.Tensor, w_fp8: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -64,18 +58,16 @@ def fp8_block_linear(x: torch.Tensor, w_fp8: torch.Tensor, w_scale: torch.Tensor
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     if x.shape[-1] != K:
         raise ValueError(f"input features {x.shape[-1]} != weight in_features {K}")
-    A.require_cuda(x, w_fp8, w_scale)
-    _same_device(x, w_fp8, w_scale, bias)
+    dev = A.cuda_index(x, w_fp8, w_scale, bias)
     lib = A.load()
-    dev = x.device
     with A.on_device(dev):
         x2 = x if x.ndim == 2 else x.reshape(-1, K)
         M = x2.shape[0]
         if M and (x2.stride(1) != 1 or (M > 1 and x2.stride(0) < K)):
             x2 = x2.contiguous()
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
         n = lib.aeoq_fp8_block_linear_workspace_size(M, N, K)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
         if not w_fp8.is_contiguous():
             w_fp8 = w_fp8.contiguous()
         if not w_scale.is_contiguous():
@@ -84,7 +76,7 @@ def fp8_block_linear(x: torch.Tensor, w_fp8: torch.Tensor, w_scale: torch.Tensor
             bias = bias.contiguous()
         A.check(lib.aeoq_fp8_block_linear(x2.data_ptr(), A.dtype_code(x.dtype), x2.stride(0) if M > 1 else K, M,
                                           w_fp8.data_ptr(), w_scale.data_ptr(), N, K, A.ptr(bias), out.data_ptr(),
-                                          code, N, ws.data_ptr(), n, A.err_ptr(dev), A.stream_ptr(dev)))
+                                          code, N, A.ptr(ws), n, A.err_ptr(dev), A.raw_stream(dev)))
     return out if x.ndim == 2 else out.reshape(*x.shape[:-1], N)
 
 
@@ -102,16 +94,13 @@ def fp8_block_linear_prequantized(x_fp8: torch.Tensor, x_scale: torch.Tensor, w_
     want = (M, -(-K // FP8_BLOCK))
     if tuple(x_scale.shape) != want or x_scale.dtype != torch.float32:
         raise ValueError(f"x_scale must be float32 of shape {want}, got {x_scale.dtype} {tuple(x_scale.shape)}")
-    A.require_cuda(x_fp8, x_scale, w_fp8, w_scale)
-    _same_device(x_fp8, x_scale, w_fp8, w_scale, bias)
-    lib = A.load()
-    dev = x_fp8.device
+    dev = A.cuda_index(x_fp8, x_scale, w_fp8, w_scale, bias)
     with A.on_device(dev):
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+        out = torch.empty((M, N), dtype=out_dtype, device=x_fp8.device)
         x_fp8, x_scale, w_fp8, w_scale = (t.contiguous() for t in (x_fp8, x_scale, w_fp8, w_scale))
         if bias is not None:
             bias = bias.contiguous()
-        A.check(lib.aeoq_fp8_block_gemm(x_fp8.data_ptr(), x_scale.data_ptr(), M, w_fp8.data_ptr(),
-                                        w_scale.data_ptr(), N, K, A.ptr(bias), out.data_ptr(), code, N,
-                                        A.err_ptr(dev), A.stream_ptr(dev)))
+        A.check(A.load().aeoq_fp8_block_gemm(x_fp8.data_ptr(), x_scale.data_ptr(), M, w_fp8.data_ptr(),
+                                             w_scale.data_ptr(), N, K, A.ptr(bias), out.data_ptr(), code, N,
+                                             A.err_ptr(dev), A.raw_stream(dev)))
     return out

@@ -130,11 +130,11 @@ def quantize_fp8_activation_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch
     dt = A.dtype_code(x.dtype)
     if dt not in (A.BF16, A.F16, A.F32):
         raise ValueError(f"unsupported dtype {x.dtype}")
-    A.require_cuda(x)
+    dev = A.cuda_index(x)
     K = x.shape[-1]
-    with A.on_device(x.device):
+    with A.on_device(dev):
         q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        s = torch.empty(*x.shape[:-1], -(-K // FP8_BLOCK), dtype=torch.float32, device=x.device)
+        s = torch.empty((*x.shape[:-1], -(-K // FP8_BLOCK)), dtype=torch.float32, device=x.device)
         if x.numel() == 0:
             return q, s
         x2 = _rows_view(x)
@@ -142,7 +142,7 @@ def quantize_fp8_activation_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch
         if rows > 1 and x2.stride(0) < K:
             x2 = x2.contiguous()                # broadcast or overlapping rows
         A.check(A.load().aeoq_fp8_block_quantize_rows(x2.data_ptr(), dt, rows, K, x2.stride(0) if rows > 1 else K,
-                                                      q.data_ptr(), K, s.data_ptr(), A.stream_ptr(x.device)))
+                                                      q.data_ptr(), K, s.data_ptr(), A.raw_stream(dev)))
     return q, s
 
 
@@ -158,14 +158,14 @@ def quantize_3d_to_fp8_block(weight: torch.Tensor) -> tuple[torch.Tensor, torch.
     dt = A.dtype_code(weight.dtype)
     if dt not in (A.BF16, A.F16, A.F32):
         raise ValueError(f"unsupported dtype {weight.dtype}")
-    A.require_cuda(weight)
+    dev = A.cuda_index(weight)
     E, N, K = weight.shape
-    with A.on_device(weight.device):
+    with A.on_device(dev):
         w = weight.contiguous()
         q = torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device=w.device)
         s = torch.empty(E, -(-N // FP8_BLOCK), -(-K // FP8_BLOCK), dtype=torch.float32, device=w.device)
         A.check(A.load().aeoq_fp8_block_quantize_weights(w.data_ptr(), dt, E, N, K, q.data_ptr(), s.data_ptr(),
-                                                         A.stream_ptr(w.device)))
+                                                         A.raw_stream(dev)))
     return q, s
 
 

@@ -61,19 +61,18 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
             raise ValueError(f"bias must have shape ({E},), got {tuple(bias.shape)}")
         if bias.dtype not in _LOGITS:
             raise ValueError(f"bias must be bfloat16, float16 or float32, got {bias.dtype}")
-        if bias.device != logits.device:
-            raise ValueError(f"bias is on {bias.device}, logits on {logits.device}")
-    A.require_cuda(logits)
-    lib = A.load()
+    dev = A.cuda_index(logits, bias)
+    if not 1 <= k <= E:
+        raise ValueError(f"route_topk: k ({k}) must be in [1, min(num_experts, 32)]")
     if logits.stride(1) != 1 or logits.stride(0) < E:
         logits = logits.contiguous()
-    with A.on_device(logits.device):
+    with A.on_device(dev):
         if bias is not None:
             bias = bias.detach().to(torch.float32).contiguous()
-        weights = torch.empty(T, k if k > 0 else 0, dtype=torch.float32, device=logits.device)
-        ids = torch.empty(T, k if k > 0 else 0, dtype=torch.int64, device=logits.device)
-        A.check(lib.aeoq_route_topk(logits.data_ptr(), A.dtype_code(logits.dtype), logits.stride(0) if T > 1 else E, T,
-                                    E, k, _SCORES[score], A.ptr(bias), n_group, topk_group,
-                                    _GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
-                                    weights.data_ptr(), ids.data_ptr(), A.stream_ptr(logits.device)))
+        weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((T, k), dtype=torch.int64, device=logits.device)
+        A.check(A.load().aeoq_route_topk(
+            logits.data_ptr(), A.dtype_code(logits.dtype), logits.stride(0) if T > 1 else E, T, E, k, _SCORES[score],
+            A.ptr(bias), n_group, topk_group, _GROUP_SCORES[group_score], int(bool(renormalize)), float(scale),
+            weights.data_ptr(), ids.data_ptr(), A.raw_stream(dev)))
     return weights, ids

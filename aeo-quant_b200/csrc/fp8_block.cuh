@@ -109,6 +109,7 @@ __device__ __forceinline__ float fb_act(int act, float x) {
 
 // Few rows of a: the weights are streamed through mma.sync (fp8_block_skinny.cu).
 constexpr int kFbSkinnyRows = 64;        // linear: rows at most
+constexpr int kFbSkinnyQuant = 8;        // linear: rows that each CTA quantizes for itself (no workspace)
 bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K);
 int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uint8_t* w, const float* sw, int64_t N,
                      int64_t K, const void* bias, void* out, int out_dt, int64_t ldc, uint8_t* q, float* qs,

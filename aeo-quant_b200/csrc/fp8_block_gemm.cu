@@ -886,7 +886,7 @@ extern "C" int aeoq_fp8_block_gemm(const uint8_t* a, const float* sa, int64_t M,
 static size_t linear_scales_at(int64_t M, int64_t K) { return (size_t)((M * K + 255) / 256 * 256); }
 
 extern "C" size_t aeoq_fp8_block_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= kFbSkinnyQuant || N <= 0 || K <= 0) return 0;
   return linear_scales_at(M, K) + (size_t)M * fb_blocks(K) * 4;
 }
 
@@ -903,8 +903,8 @@ extern "C" int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int6
   AEOQ_REQUIRE(x && w && sw && out, AEOQ_ERR_INVALID, "fp8_block_linear: null pointer");
   AEOQ_REQUIRE((uintptr_t)w % 16 == 0, AEOQ_ERR_INVALID, "fp8_block_linear: weights must be 16-byte aligned");
   const size_t need = aeoq_fp8_block_linear_workspace_size(M, N, K);
-  AEOQ_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 256 == 0, AEOQ_ERR_WORKSPACE,
-               "fp8_block_linear: a 256-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  AEOQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 256 == 0),
+               AEOQ_ERR_WORKSPACE, "fp8_block_linear: a 256-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   cudaStream_t st = (cudaStream_t)stream;
   uint8_t* q = reinterpret_cast<uint8_t*>(workspace);
   float* s = reinterpret_cast<float*>(q + linear_scales_at(M, K));

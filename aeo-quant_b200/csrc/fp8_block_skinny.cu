@@ -57,14 +57,15 @@ struct SkWeights {
 
 // This lane's 32 values of column g in one block, quantized: codes and the
 // block's scale. v: the lane's piece (null: zeros); n: values of it that exist
-// (a multiple of 16).
-template <int DT>
+// (a multiple of 16); VEC: pieces are 16-byte aligned.
+template <int DT, bool VEC>
 __device__ __forceinline__ void sk_quantize(const typename In<DT>::T* v, int64_t n, uint32_t (&c)[8], float& scale) {
   FbEight<DT> e[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (v && 8 * i < n) {
-      e[i].load(v + 8 * i);
+      if constexpr (VEC) e[i].load(v + 8 * i);
+      else e[i].load_some(v + 8 * i, 8);
     } else {
       e[i].zero();
     }
@@ -116,7 +117,7 @@ struct SkLinear {
 
 // CTA: 16 output columns, all M rows in NB groups of 8. QUANT: quantize x here
 // (NB = 1); else read codes.
-template <int DT, bool QUANT, int NB>
+template <int DT, bool QUANT, bool VEC, int NB>
 __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p) {
   __shared__ float part[kSkWarps][32][4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
         float xs = 0.0f, d[4];
         if constexpr (QUANT) {
           const auto* x = reinterpret_cast<const typename In<DT>::T*>(p.x);
-          sk_quantize<DT>(m < p.M ? x + m * p.ldx + k0 : nullptr, p.K - k0, c, xs);
+          sk_quantize<DT, VEC>(m < p.M ? x + m * p.ldx + k0 : nullptr, p.K - k0, c, xs);
         } else {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -182,7 +183,10 @@ bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K) { return M <= kFbSk
 
 template <int DT>
 static int launch_quant(const SkLinear& p, cudaStream_t st) {
-  sk_linear_kernel<DT, true, 1><<<(unsigned)((p.N + 15) / 16), kSkThreads, 0, st>>>(p);
+  const bool vec = (uintptr_t)p.x % 16 == 0 && (p.ldx * (int64_t)sizeof(typename In<DT>::T)) % 16 == 0;
+  const unsigned grid = (unsigned)((p.N + 15) / 16);
+  if (vec) sk_linear_kernel<DT, true, true, 1><<<grid, kSkThreads, 0, st>>>(p);
+  else sk_linear_kernel<DT, true, false, 1><<<grid, kSkThreads, 0, st>>>(p);
   return check_launch("sk_linear_kernel");
 }
 
@@ -202,8 +206,7 @@ int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uin
   p.out = out;
   p.out_dt = out_dt;
   p.ldc = ldc;
-  const int es = dtype == AEOQ_F32 ? 4 : 2;
-  if (x && M <= 8 && (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0) {
+  if (x && M <= kFbSkinnyQuant) {
     if (dtype == AEOQ_BF16) return launch_quant<AEOQ_BF16>(p, st);
     if (dtype == AEOQ_F16) return launch_quant<AEOQ_F16>(p, st);
     return launch_quant<AEOQ_F32>(p, st);
@@ -215,10 +218,10 @@ int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uin
   p.q = q;
   p.qs = qs;
   const unsigned grid = (unsigned)((N + 15) / 16);
-  if (M <= 8) sk_linear_kernel<AEOQ_BF16, false, 1><<<grid, kSkThreads, 0, st>>>(p);
-  else if (M <= 16) sk_linear_kernel<AEOQ_BF16, false, 2><<<grid, kSkThreads, 0, st>>>(p);
-  else if (M <= 32) sk_linear_kernel<AEOQ_BF16, false, 4><<<grid, kSkThreads, 0, st>>>(p);
-  else sk_linear_kernel<AEOQ_BF16, false, 8><<<grid, kSkThreads, 0, st>>>(p);
+  if (M <= 8) sk_linear_kernel<AEOQ_BF16, false, true, 1><<<grid, kSkThreads, 0, st>>>(p);
+  else if (M <= 16) sk_linear_kernel<AEOQ_BF16, false, true, 2><<<grid, kSkThreads, 0, st>>>(p);
+  else if (M <= 32) sk_linear_kernel<AEOQ_BF16, false, true, 4><<<grid, kSkThreads, 0, st>>>(p);
+  else sk_linear_kernel<AEOQ_BF16, false, true, 8><<<grid, kSkThreads, 0, st>>>(p);
   return check_launch("sk_linear_kernel");
 }
 

@@ -59,7 +59,7 @@ def test_linear_c_refusals(lib):
     assert n >= 33 * 272 + 33 * 3 * 4 and lib.aeoq_fp8_block_linear_workspace_size(0, 256, 256) == 0
 
     def linear(ws=None, bytes_=0, ldx=256, dt=0):
-        return lib.aeoq_fp8_block_linear(16, dt, ldx, 4, 16, 16, 256, 256, None, 16, 0, 256, ws, bytes_, None, None)
+        return lib.aeoq_fp8_block_linear(16, dt, ldx, 40, 16, 16, 256, 256, None, 16, 0, 256, ws, bytes_, None, None)
     assert linear() == -3 and b"workspace" in lib.aeoq_last_error()
     assert linear(ws=256, bytes_=100) == -3
     assert linear(ws=257, bytes_=1 << 20) == -3

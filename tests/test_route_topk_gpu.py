@@ -178,9 +178,10 @@ def test_strides_offsets_and_empty():
 
 
 def test_refused_on_gpu():
+    from aeo_quant_b200 import AeoqError
     from aeo_quant_b200.gpu.routing import route_topk
     l = torch.zeros(2, 16, device="cuda")
-    with pytest.raises(ValueError, match="bias is on cpu"):
+    with pytest.raises(AeoqError, match="CUDA tensors only"):
         route_topk(l, 2, bias=torch.zeros(16))
     for bad in (0, -1, 17):
         with pytest.raises(ValueError, match="route_topk: k"):
