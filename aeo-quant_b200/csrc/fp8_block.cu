@@ -14,14 +14,17 @@ constexpr int kFbRowWarps = 8;
 
 // One warp per row and run of `chunk` blocks. VEC: rows, their pieces of 8
 // and the code rows are aligned for wide accesses and K % 8 == 0.
-template <int DT, bool VEC>
+// `to` (VEC only): instead of to row r the codes and scales of row r go to rows
+// to[r * k] .. to[r * k + k - 1], those that are not negative.
+template <int DT, bool VEC, bool SCATTER>
 __global__ void __launch_bounds__(32 * kFbRowWarps) fb_rows_kernel(
-    const typename In<DT>::T* __restrict__ x, int64_t rows, int64_t K, int64_t ld, const int* __restrict__ idx,
-    const int* __restrict__ n_rows, int chunk, uint8_t* __restrict__ q, int64_t q_ld, float* __restrict__ scale) {
+    const typename In<DT>::T* __restrict__ x, int64_t rows, int64_t K, int64_t ld,
+    int chunk, uint8_t* __restrict__ q, int64_t q_ld, float* __restrict__ scale, const int* __restrict__ to, int k) {
+  pdl_trigger();      // a dependent that asked for it may start its own loads
   const int64_t r = blockIdx.x * (int64_t)kFbRowWarps + (threadIdx.x >> 5);
-  if (r >= rows || (n_rows && r >= *n_rows)) return;
+  if (r >= rows) return;
   const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
-  const typename In<DT>::T* xr = x + (idx ? (int64_t)idx[r] : r) * ld;
+  const typename In<DT>::T* xr = x + r * ld;
   uint8_t* qr = q + r * q_ld;
   const int nb = (int)fb_blocks(K);
   float* sr = scale + r * nb;
@@ -52,7 +55,16 @@ __global__ void __launch_bounds__(32 * kFbRowWarps) fb_rows_kernel(
 #pragma unroll
     for (int u = 1; u < U; ++u) mine = (sub & 3) == u ? key[u] : mine;
     const float2 s = fb_scales(FbEight<DT>::key_value(mine));
-    if (sub < U && b0 + 2 * sub + half < b_end) sr[b0 + 2 * sub + half] = s.y;
+    if (sub < U && b0 + 2 * sub + half < b_end) {
+      if constexpr (SCATTER) {
+        for (int j = 0; j < k; ++j) {
+          const int d = __ldg(to + r * k + j);
+          if (d >= 0) scale[(int64_t)d * nb + b0 + 2 * sub + half] = s.y;
+        }
+      } else {
+        sr[b0 + 2 * sub + half] = s.y;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int b = b0 + 2 * u + half;
@@ -60,7 +72,12 @@ __global__ void __launch_bounds__(32 * kFbRowWarps) fb_rows_kernel(
       const float inv = __shfl_sync(0xFFFFFFFFu, s.x, (lane & 16) | u);
       if (b >= b_end || k0 >= K) continue;
       const uint2 c = fb_codes8(v[u], inv);
-      if (VEC) {
+      if (SCATTER) {
+        for (int j = 0; j < k; ++j) {
+          const int d = __ldg(to + r * k + j);
+          if (d >= 0) *reinterpret_cast<uint2*>(q + (int64_t)d * q_ld + k0) = c;
+        }
+      } else if (VEC) {
         *reinterpret_cast<uint2*>(qr + k0) = c;
       } else {
 #pragma unroll
@@ -121,8 +138,8 @@ __global__ void __launch_bounds__(256) fb_weights_kernel(const typename In<DT>::
 }
 
 template <int DT>
-static int launch_rows(const void* x, int64_t rows, int64_t K, int64_t ld, const int* idx, const int* n_rows,
-                       uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st) {
+static int launch_rows(const void* x, int64_t rows, int64_t K, int64_t ld, uint8_t* q,
+                       int64_t q_ld, float* scale, cudaStream_t st) {
   using T = typename In<DT>::T;
   const bool vec = K % 8 == 0 && (uintptr_t)x % 16 == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0 &&
                    (uintptr_t)q % 8 == 0 && q_ld % 8 == 0;
@@ -134,22 +151,30 @@ static int launch_rows(const void* x, int64_t rows, int64_t K, int64_t ld, const
   if (groups * 2 <= device_sm_count()) chunk = groups * ((nb + 7) / 8) >= device_sm_count() ? 8 : 2;
   dim3 grid((unsigned)groups, (unsigned)((nb + chunk - 1) / chunk));
   if (vec)
-    fb_rows_kernel<DT, true><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld, idx,
-                                                                n_rows, (int)chunk, q, q_ld, scale);
+    fb_rows_kernel<DT, true, false><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld,
+                                                                (int)chunk, q, q_ld, scale, nullptr, 0);
   else
-    fb_rows_kernel<DT, false><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld, idx,
-                                                                 n_rows, (int)chunk, q, q_ld, scale);
+    fb_rows_kernel<DT, false, false><<<grid, 32 * kFbRowWarps, 0, st>>>(reinterpret_cast<const T*>(x), rows, K, ld,
+                                                                 (int)chunk, q, q_ld, scale, nullptr, 0);
   return check_launch("fb_rows_kernel");
 }
 
-int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, const int* idx,
-                     const int* n_rows, uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st) {
+int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, uint8_t* q, int64_t q_ld,
+                     float* scale, cudaStream_t st) {
   switch (dtype) {
-    case AEOQ_BF16: return launch_rows<AEOQ_BF16>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
-    case AEOQ_F16: return launch_rows<AEOQ_F16>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
-    case AEOQ_F32: return launch_rows<AEOQ_F32>(x, rows, K, ld, idx, n_rows, q, q_ld, scale, st);
+    case AEOQ_BF16: return launch_rows<AEOQ_BF16>(x, rows, K, ld, q, q_ld, scale, st);
+    case AEOQ_F16: return launch_rows<AEOQ_F16>(x, rows, K, ld, q, q_ld, scale, st);
+    case AEOQ_F32: return launch_rows<AEOQ_F32>(x, rows, K, ld, q, q_ld, scale, st);
   }
   return set_error(AEOQ_ERR_INVALID, "fp8_block_quantize_rows: unsupported dtype %d", dtype);
+}
+
+int fb_quantize_rows_to(const void* x, int64_t rows, int64_t K, const int* to, int k, uint8_t* q, float* scale,
+                        cudaStream_t st) {
+  const int64_t groups = (rows + kFbRowWarps - 1) / kFbRowWarps;
+  fb_rows_kernel<AEOQ_BF16, true, true><<<dim3((unsigned)groups, 1), 32 * kFbRowWarps, 0, st>>>(
+      reinterpret_cast<const __nv_bfloat16*>(x), rows, K, K, (int)fb_blocks(K), q, K, scale, to, k);
+  return check_launch("fb_rows_kernel");
 }
 
 template <int DT>
@@ -177,7 +202,7 @@ extern "C" int aeoq_fp8_block_quantize_rows(const void* x, int dtype, int64_t ro
                "fp8_block_quantize_rows: K at most 2^24, rows at most 2^33");
   if (rows == 0 || K == 0) return AEOQ_OK;
   AEOQ_REQUIRE(x && q && scale, AEOQ_ERR_INVALID, "fp8_block_quantize_rows: null pointer");
-  return fb_quantize_rows(x, dtype, rows, K, ld, nullptr, nullptr, q, q_ld, scale, (cudaStream_t)stream);
+  return fb_quantize_rows(x, dtype, rows, K, ld, q, q_ld, scale, (cudaStream_t)stream);
 }
 
 extern "C" int aeoq_fp8_block_quantize_weights(const void* x, int dtype, int64_t num_experts, int64_t N, int64_t K,

@@ -108,7 +108,6 @@ __device__ __forceinline__ float fb_act(int act, float x) {
 }
 
 // Few rows of a: the weights are streamed through mma.sync (fp8_block_skinny.cu).
-constexpr int kFbSkinnyRows = 64;        // linear: rows at most
 constexpr int kFbSkinnyQuant = 8;        // linear: rows that each CTA quantizes for itself (no workspace)
 bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K);
 int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uint8_t* w, const float* sw, int64_t N,
@@ -119,9 +118,12 @@ int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt
                       const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,
                       int64_t I, int act, float* h, void* out, cudaStream_t st);
 
-// Rows [0, rows) of x (or x[idx[r]], r < *n_rows) quantized per 128 values; their
-// scales (rows, ceil(K / 128)).
-int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, const int* idx,
-                     const int* n_rows, uint8_t* q, int64_t q_ld, float* scale, cudaStream_t st);
+// Rows of x quantized per 128 values; their scales (rows, ceil(K / 128)).
+int fb_quantize_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ld, uint8_t* q, int64_t q_ld,
+                     float* scale, cudaStream_t st);
+// The same for contiguous, 16-byte aligned bf16 rows with K % 8 == 0; row r goes
+// to the rows to[r * k] .. to[r * k + k - 1] that are not negative.
+int fb_quantize_rows_to(const void* x, int64_t rows, int64_t K, const int* to, int k, uint8_t* q, float* scale,
+                        cudaStream_t st);
 
 }  // namespace aeoq

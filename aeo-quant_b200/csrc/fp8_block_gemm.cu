@@ -56,6 +56,7 @@ struct FbParams {
   const float* sa;        // (rows of a, KB): a row's scales share lines that stay in L1 for several K
                           // steps (the other order, 8192 x 8192 x 8192: 689 against 521 us)
   const float* sw;        // (E, NB, KB)
+  const int* row_src;     // few rows, GLU: sorted row r is row row_src[r] of a (a token's)
   const int* grp_off;     // grouped: rows [grp_off[e], grp_off[e + 1]) are expert e's; null: dense
   const int* tile_off;    // grouped: row tiles before expert e's, E + 1 values
   int64_t tiles_m;        // dense
@@ -505,6 +506,9 @@ static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbPar
 //
 // Tile: 256 rows of w as two MMAs of 128 (GLU: 128 gate rows and the 128 up
 // rows that go with them; store: 256 consecutive ones) times 32 tokens.
+// GLU gathers its tokens' rows where they are (a gather4 of four rows per
+// lane; for tiles of 128 rows that takes too long: 460 against 267 us at 4096
+// tokens, so there the quantizer writes a row for each of a token's experts).
 //   warp 0 TMA, warp 1 MMA and TMEM, warps 4-11 scaling and epilogue: four
 //   warps with tokens 0-15, four with tokens 16-31
 struct FbFewLayout {
@@ -522,6 +526,15 @@ struct FbFewLayout {
   static constexpr size_t kBytes = 1024 + (size_t)kStages * kStage + sizeof(Ctl);
   static constexpr uint32_t kTmemCols = 128;   // 2 buffers x 2 MMAs x 32 tokens
 };
+
+// Source rows of the sorted rows r0 .. r0 + 3 of a tile (past its last one:
+// the first, whose products are not used).
+__device__ __forceinline__ int4 fb_rows4(const FbParams& p, const FbTile& ti, int r0) {
+  int v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __ldg(p.row_src + ti.row0 + (r0 + i < ti.rows ? r0 + i : 0));
+  return make_int4(v[0], v[1], v[2], v[3]);
+}
 
 template <int EPI>
 __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __grid_constant__ CUtensorMap tmW,
@@ -578,6 +591,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
       const int w0 = (int)(ti.expert * p.N + ti.n0);
       // boxes of 64 rows of w: those that hold an output column
       const int left = (int)((EPI == kFbGlu ? p.I : p.N) - ti.n0), boxes = min(kWide / 64, (left + 63) / 64);
+      int4 src = make_int4(0, 0, 0, 0);
+      if (EPI == kFbGlu) src = fb_rows4(p, ti, 4 * (lane & 7));
       for (int kb = 0; kb < KB; ++kb, ++g) {
         const uint32_t s = g % L::kStages, ph = (g / L::kStages) & 1;
         if (!sm100::mbar_wait(&sh->empty[s], ph ^ 1, p.err, 81)) { alive = false; break; }
@@ -589,8 +604,10 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
             if (EPI == kFbGlu)
               sm100::tma_load_2d(st + 16384 + i * 8192, &tmW, kb * 128, w0 + (int)p.I + 64 * i, &sh->full[s]);
           }
-          sm100::tma_load_2d(st + L::kA, &tmB, kb * 128, (int)ti.row0, &sh->full[s]);
+          if (EPI == kFbStore) sm100::tma_load_2d(st + L::kA, &tmB, kb * 128, (int)ti.row0, &sh->full[s]);
         }
+        if (EPI == kFbGlu && lane < L::kTok / 4)
+          sm100::tma_gather4(base + s * L::kStage + L::kA + lane * 512, &tmB, kb * 128, src, &sh->full[s]);
         __syncwarp();
       }
     }
@@ -634,7 +651,9 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
       }
       // lane j's token scale; the two MMAs' weight scales (rows past the last
       // one take its scale, their sums are not used)
-      const float* sa = p.sa + (ti.row0 + tok0 + min(lane & 15, n_tok - 1)) * KB;
+      int64_t r = ti.row0 + tok0 + min(lane & 15, n_tok - 1);
+      if (EPI == kFbGlu) r = __ldg(p.row_src + r);
+      const float* sa = p.sa + r * KB;
       const float* se = p.sw + ti.expert * p.NB * KB;
       const int64_t c0 = min(ti.n0 + f, p.N - 1), c1 = min((EPI == kFbGlu ? p.I : 128) + ti.n0 + f, p.N - 1);
       const float *sw0 = se + (c0 / kFbBlock) * KB, *sw1 = se + (c1 / kFbBlock) * KB;
@@ -718,7 +737,7 @@ static int launch_few(const uint8_t* a, int64_t a_rows, const uint8_t* w, const 
   CUtensorMap tw, tb;
   int rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, 64, true);
   if (rc) return rc;
-  rc = make_tmap_bytes(&tb, a, a_rows, p.K, p.K, 128, L::kTok, true);
+  rc = make_tmap_bytes(&tb, a, a_rows, p.K, p.K, 128, EPI == kFbGlu ? 1 : L::kTok, true);
   if (rc) return rc;
   AEOQ_REQUIRE(max_tiles <= 0x7FFFFFFF, AEOQ_ERR_INVALID, "fp8_block_few: too many tiles");
   rc = func_smem_attr((const void*)fp8_block_few_kernel<EPI>, L::kBytes, -1, "fp8_block_few");
@@ -744,34 +763,54 @@ static int gemm_dense(const uint8_t* a, const float* sa, int64_t M, const uint8_
   p.ldc = ldc;
   p.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
   p.err = err;
-  // Tiles of 256 columns once they fill the SMs; below that 128, of which
-  // there are more.
+  // A K step of a tile of 128 columns takes not half of but 5/6 of what one of
+  // 256 takes (the hand-over of the accumulators, not the MMAs, bounds it), so
+  // the narrow tiles pay only where they take fewer rounds of CTAs: 1024 x 1408 x
+  // 2816 24.6 against 28.7 us, 2048 x 1408 x 2816 34.8 against 28.7.
+  const int64_t sms = device_sm_count();
   p.tiles_m = (M + 127) / 128;
   p.tiles_n = (int)((N + 255) / 256);
-  if (p.tiles_m * p.tiles_n >= device_sm_count())
-    return launch_gemm<256, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
+  const int64_t wide = p.tiles_m * p.tiles_n, narrow = p.tiles_m * ((N + 127) / 128);
+  if (6 * ((wide + sms - 1) / sms) < 5 * ((narrow + sms - 1) / sms))
+    return launch_gemm<256, kFbStore>(a, M, w, p, wide, st);
   p.tiles_n = (int)((N + 127) / 128);
-  return launch_gemm<128, kFbStore>(a, M, w, p, p.tiles_m * p.tiles_n, st);
+  return launch_gemm<128, kFbStore>(a, M, w, p, narrow, st);
 }
 
 // ---------------------------------------------------------------- experts
-// Pairs (token, slot) sorted by expert: a counting sort in one CTA.
+// Pairs (token, slot) sorted by expert: a counting sort by one cluster of
+// CTAs, each with its slice of the pairs.
 //   grp_off[e]   first row of expert e        (E + 1 values)
 //   tile_off[e]  tiles of `tile` rows before expert e (E + 1 values)
 //   row_tok[r]   token of sorted row r;  pair_row[i]  row of pair i, or -1
+// The order of an expert's rows within one CTA's slice is arbitrary; each row
+// is computed by itself and the sum over a token's slots goes by slot.
+constexpr int kFbSortCtas = 8;
 __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_dt, int64_t n_pairs, int k, int E,
-                                                       int tile, int* grp_off, int* tile_off, int* row_tok, int* pair_row) {
+                                                       int tile, int* grp_off, int* tile_off, int* row_tok,
+                                                       int* pair_row) {
   __shared__ int cnt[kFbMaxExperts], fill[kFbMaxExperts];
   __shared__ int s_row[32], s_tile[32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, ctas = gridDim.x, rank = blockIdx.x;
+  const int64_t slice = (n_pairs + ctas - 1) / ctas, beg = rank * slice, end = min(n_pairs, beg + slice);
   cnt[t] = 0;
   __syncthreads();
-  for (int64_t i = t; i < n_pairs; i += 1024) {
+  for (int64_t i = beg + t; i < end; i += 1024) {
     const int64_t e = load_index(ids, ids_dt, i);
     if (e >= 0 && e < E) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
-  const int c = cnt[t], d = (c + tile - 1) / tile;      // experts past E count 0
+  int c = cnt[t], before = 0;      // all CTAs' pairs of expert t, those of lower ranks
+  if (ctas > 1) {
+    sm100::cluster_sync();
+    c = 0;
+    for (int r = 0; r < ctas; ++r) {
+      const int v = __float_as_int(sm100::ld_dsmem_f32(sm100::dsmem_addr(&cnt[t], r)));
+      c += v;
+      before += r < rank ? v : 0;
+    }
+  }
+  const int d = (c + tile - 1) / tile;      // experts past E count 0
   int r = c, q = d;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -781,14 +820,14 @@ __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_
   if (lane == 31) { s_row[warp] = r; s_tile[warp] = q; }
   __syncthreads();
   for (int w = 0; w < warp; ++w) { r += s_row[w]; q += s_tile[w]; }
-  fill[t] = r - c;
-  if (t < E) {
+  fill[t] = r - c + before;
+  if (t < E && rank == 0) {
     grp_off[t] = r - c;
     tile_off[t] = q - d;
     if (t == E - 1) { grp_off[E] = r; tile_off[E] = q; }
   }
   __syncthreads();
-  for (int64_t i = t; i < n_pairs; i += 1024) {
+  for (int64_t i = beg + t; i < end; i += 1024) {
     const int64_t e = load_index(ids, ids_dt, i);
     int at = -1;
     if (e >= 0 && e < E) {
@@ -797,6 +836,25 @@ __global__ void __launch_bounds__(1024) fb_sort_kernel(const void* ids, int ids_
     }
     pair_row[i] = at;
   }
+  if (ctas > 1) sm100::cluster_sync();      // the others have read this CTA's counts
+}
+
+static int launch_sort(const void* ids, int ids_dt, int64_t n_pairs, int k, int E, int tile, int* grp_off,
+                       int* tile_off, int* row_tok, int* pair_row, cudaStream_t st) {
+  // one CTA up to 4096 pairs (4 per thread), else a cluster
+  const int ctas = n_pairs > 4096 ? kFbSortCtas : 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, fb_sort_kernel, ids, ids_dt, n_pairs, k, E, tile, grp_off, tile_off, row_tok, pair_row);
+  return check_launch("fb_sort_kernel");
 }
 
 // out[t] = sum over slots j, in order, of weights[t][j] * y[pair_row[t][j]], in
@@ -825,6 +883,11 @@ __global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __
   }
 }
 
+// Weights on the MMA's rows up to 40 rows per expert: at 128 experts, top-8, H =
+// 2816, I = 704 (cold L2) 64 tokens take 170 us that way and 228 the other,
+// 512 tokens (32 rows) 205 and 244, 1024 tokens (64 rows) 328 and 260.
+static bool fb_few(int64_t pairs, int64_t experts) { return pairs <= 40 * experts; }
+
 // Workspace: of the grouped forward, or of that for few tokens (h alone).
 struct FbExpertsWs {
   size_t grp_off = 0, tile_off = 0, row_tok = 0, pair_row = 0, xq = 0, xs = 0, hq = 0, hs = 0, y = 0, h = 0, bytes = 0;
@@ -845,8 +908,9 @@ struct FbExpertsWs {
     tile_off = take(4 * (E + 1));
     row_tok = take(4 * P);
     pair_row = take(4 * P);
-    xq = take(P * H);
-    xs = take(4 * P * fb_blocks(H));
+    const int64_t rows = fb_few(P, E) ? T : P;
+    xq = take(rows * H);
+    xs = take(4 * rows * fb_blocks(H));
     hq = take(P * I);
     hs = take(4 * P * fb_blocks(I));
     y = take(2 * P * H);
@@ -910,7 +974,7 @@ extern "C" int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int6
   float* s = reinterpret_cast<float*>(q + linear_scales_at(M, K));
   if (fb_linear_skinny_takes(M, N, K))
     return fb_linear_skinny(x, dtype, ldx, M, w, sw, N, K, bias, out, out_dtype, ldc, q, s, st);
-  rc = fb_quantize_rows(x, dtype, M, K, ldx, nullptr, nullptr, q, K, s, st);
+  rc = fb_quantize_rows(x, dtype, M, K, ldx, q, K, s, st);
   if (rc) return rc;
   return gemm_dense(q, s, M, w, sw, N, K, bias, out, out_dtype, ldc, err_word, st);
 }
@@ -957,17 +1021,13 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   if (fb_experts_skinny_takes(T, k, E, H, I))
     return fb_experts_skinny(hidden, T, top_k_index, idx_dtype, top_k_weights, k, gate_up, gate_up_scale, down,
                              down_scale, E, H, I, activation, floats(l.h), out, st);
-  // Weights on the MMA's rows up to 40 rows per expert: at 128 experts, top-8,
-  // H = 2816, I = 704 (cold L2) 64 tokens take 170 us that way and 228 the
-  // other, 512 tokens (32 rows) 205 and 244, 1024 tokens (64 rows) 328 and 260.
-  const bool few = P <= 40 * E;
+  const bool few = fb_few(P, E);
   const int tile = few ? FbFewLayout::kTok : 128;
-  fb_sort_kernel<<<1, 1024, 0, st>>>(top_k_index, idx_dtype, P, (int)k, (int)E, tile, ints(l.grp_off), ints(l.tile_off),
-                                     ints(l.row_tok), ints(l.pair_row));
-  int rc = check_launch("fb_sort_kernel");
+  int rc = launch_sort(top_k_index, idx_dtype, P, (int)k, (int)E, tile, ints(l.grp_off), ints(l.tile_off),
+                       ints(l.row_tok), ints(l.pair_row), st);
   if (rc) return rc;
-  rc = fb_quantize_rows(hidden, AEOQ_BF16, P, H, H, ints(l.row_tok), ints(l.grp_off) + E, ws + l.xq, H,
-                        floats(l.xs), st);
+  rc = few ? fb_quantize_rows(hidden, AEOQ_BF16, T, H, H, ws + l.xq, H, floats(l.xs), st)
+           : fb_quantize_rows_to(hidden, T, H, ints(l.pair_row), (int)k, ws + l.xq, floats(l.xs), st);
   if (rc) return rc;
   const int64_t max_tiles = std::min<int64_t>(P, (P + tile - 1) / tile + E);
   FbParams p{};
@@ -979,6 +1039,7 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   p.E = (int)E;
   p.sa = floats(l.xs);
   p.sw = gate_up_scale;
+  p.row_src = ints(l.row_tok);
   p.grp_off = ints(l.grp_off);
   p.tile_off = ints(l.tile_off);
   p.tiles_n = (int)fb_blocks(I);
@@ -989,7 +1050,7 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   p.hs = floats(l.hs);
   p.hs_ld = fb_blocks(I);
   p.err = err_word;
-  rc = few ? launch_few<kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st)
+  rc = few ? launch_few<kFbGlu>(ws + l.xq, T, gate_up, p, max_tiles * p.tiles_n, st)
            : launch_gemm<256, kFbGlu>(ws + l.xq, P, gate_up, p, max_tiles * p.tiles_n, st);
   if (rc) return rc;
   FbParams d{};
@@ -1011,8 +1072,7 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   rc = few ? launch_few<kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st)
            : launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
   if (rc) return rc;
-  const int64_t pieces = T * (H / 8);
-  const unsigned blocks = (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)device_sm_count() * 16);
+  const unsigned blocks = (unsigned)std::min<int64_t>((T * (H / 8) + 255) / 256, (int64_t)device_sm_count() * 16);
   fb_combine_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(ws + l.y), ints(l.pair_row),
                                             top_k_weights, T, (int)k, H, reinterpret_cast<__nv_bfloat16*>(out));
   return check_launch("fb_combine_kernel");

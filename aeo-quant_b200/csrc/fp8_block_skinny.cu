@@ -104,6 +104,27 @@ __device__ __forceinline__ float sk_sum(const float (*part)[32][4], int row, int
   return s;
 }
 
+// One warp's codes of a row of one block, four values per lane: written to
+// `codes` (128 bytes) in shared memory, the scale returned to every lane.
+__device__ __forceinline__ float sk_quantize_warp(const float (&v)[4], uint8_t* codes) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) key = max(key, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  key = __reduce_max_sync(0xFFFFFFFFu, key);
+  const float2 s = fb_scales(__uint_as_float(key));
+  reinterpret_cast<uint32_t*>(codes)[lane] = fb_codes4(v[0] * s.x, v[1] * s.x, v[2] * s.x, v[3] * s.x);
+  return s.y;
+}
+
+// A lane's piece of a row's codes in shared memory, for every column alike.
+__device__ __forceinline__ void sk_codes(const uint8_t* codes, uint32_t (&c)[8]) {
+  const uint4* q = reinterpret_cast<const uint4*>(codes + 32 * (threadIdx.x & 3));
+  const uint4 a = q[0], b = q[1];
+  c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+  c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
+}
+
 // ------------------------------------------------------------------ linear
 struct SkLinear {
   const void* x; int64_t ldx;          // M rows of the input ...
@@ -126,6 +147,7 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
   const uint8_t* w1 = n0 + 8 + g < p.N ? p.w + (n0 + 8 + g) * p.K : nullptr;
   const float* sw = p.sw + (n0 / kFbBlock) * p.KB;     // 16 rows lie in one block row
   float acc[NB][4] = {};
+  if (!QUANT && warp >= p.KB) pdl_wait();
   for (int kb0 = warp; kb0 < p.KB; kb0 += kSkWarps * kSkAhead) {
     SkWeights w[kSkAhead];
     float s[kSkAhead];
@@ -135,6 +157,8 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
       w[u].load(w0, w1, (int64_t)kb * kFbBlock + 32 * t, kb < p.KB ? p.K : 0);
       s[u] = kb < p.KB ? __ldg(sw + kb) : 0.0f;
     }
+    // the codes come from a kernel that may still be running
+    if (!QUANT && kb0 == warp) pdl_wait();
 #pragma unroll
     for (int u = 0; u < kSkAhead; ++u) {
       const int kb = kb0 + u * kSkWarps;
@@ -142,6 +166,7 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
       const int64_t k0 = (int64_t)kb * kFbBlock + 32 * t;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
+        if (b && 8 * b >= p.M) break;
         const int64_t m = 8 * b + g;
         uint32_t c[8];
         float xs = 0.0f, d[4];
@@ -152,11 +177,11 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const bool in = m < p.M && k0 + 16 * i < p.K;
-            const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(p.q + m * p.K + k0 + 16 * i))
+            const uint4 v = in ? __ldcg(reinterpret_cast<const uint4*>(p.q + m * p.K + k0 + 16 * i))
                                : make_uint4(0u, 0u, 0u, 0u);
             c[4 * i] = v.x; c[4 * i + 1] = v.y; c[4 * i + 2] = v.z; c[4 * i + 3] = v.w;
           }
-          xs = m < p.M ? __ldg(p.qs + m * p.KB + kb) : 0.0f;
+          xs = m < p.M ? __ldcg(p.qs + m * p.KB + kb) : 0.0f;
         }
         w[u].dot(d, c);
         sk_add(acc[b], d, xs, s[u], s[u]);
@@ -165,6 +190,7 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
+    if (b && 8 * b >= p.M) break;
     if (b) __syncthreads();
     *reinterpret_cast<float4*>(part[warp][lane]) = make_float4(acc[b][0], acc[b][1], acc[b][2], acc[b][3]);
     __syncthreads();
@@ -179,7 +205,102 @@ __global__ void __launch_bounds__(kSkThreads) sk_linear_kernel(const SkLinear p)
   }
 }
 
-bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K) { return M <= kFbSkinnyRows; }
+// One row: as above, but a block of x is quantized by the whole warp, four
+// values per lane, and every column of the MMA is that row (1 x 8192 x 8192:
+// a lane of eight quantizing 32 values for itself took 28.7 us).
+template <int DT, bool VEC, int NW>
+__global__ void __launch_bounds__(32 * NW, 20 / NW) sk_row_kernel(const SkLinear p) {
+  __shared__ float part[NW][16];
+  __shared__ __align__(16) uint8_t codes[NW][kSkAhead][128];
+  using Tp = typename In<DT>::T;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const uint8_t* w0 = n0 + g < p.N ? p.w + (n0 + g) * p.K : nullptr;
+  const uint8_t* w1 = n0 + 8 + g < p.N ? p.w + (n0 + 8 + g) * p.K : nullptr;
+  const float* sw = p.sw + (n0 / kFbBlock) * p.KB;
+  const Tp* x = reinterpret_cast<const Tp*>(p.x) + 4 * lane;
+  float acc0 = 0.0f, acc1 = 0.0f;
+  for (int kb0 = warp; kb0 < p.KB; kb0 += NW * kSkAhead) {
+    SkWeights w[kSkAhead];
+    float s[kSkAhead];
+    __align__(16) Tp xv[kSkAhead][4];
+#pragma unroll
+    for (int u = 0; u < kSkAhead; ++u) {
+      const int kb = kb0 + u * NW;
+      const bool in = kb < p.KB;
+      const Tp* xk = x + (int64_t)kb * kFbBlock;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xv[u][i] = Tp(0.0f);
+      if (in && (int64_t)kb * kFbBlock + 4 * lane < p.K) {
+        if constexpr (!VEC) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[u][i] = xk[i];
+        } else if constexpr (sizeof(Tp) == 2) {
+          *reinterpret_cast<uint2*>(xv[u]) = __ldg(reinterpret_cast<const uint2*>(xk));
+        } else {
+          *reinterpret_cast<uint4*>(xv[u]) = __ldg(reinterpret_cast<const uint4*>(xk));
+        }
+      }
+      w[u].load(w0, w1, (int64_t)kb * kFbBlock + 32 * t, in ? p.K : 0);
+      s[u] = in ? __ldg(sw + kb) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kSkAhead; ++u) {
+      const float v[4] = {In<DT>::to_f(xv[u][0]), In<DT>::to_f(xv[u][1]), In<DT>::to_f(xv[u][2]),
+                          In<DT>::to_f(xv[u][3])};
+      s[u] *= sk_quantize_warp(v, codes[warp][u]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kSkAhead; ++u) {
+      if (kb0 + u * NW >= p.KB) break;
+      uint32_t c[8];
+      float d[4];
+      sk_codes(codes[warp][u], c);
+      w[u].dot(d, c);
+      acc0 = fmaf(d[0], s[u], acc0);
+      acc1 = fmaf(d[2], s[u], acc1);
+    }
+    __syncwarp();
+  }
+  if (t == 0) {
+    part[warp][g] = acc0;
+    part[warp][g + 8] = acc1;
+  }
+  __syncthreads();
+  const int64_t n = n0 + threadIdx.x;
+  if (threadIdx.x < 16 && n < p.N) {
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) y += part[w][threadIdx.x];
+    if (p.bias) y += __bfloat162float(p.bias[n]);
+    if (p.out_dt == AEOQ_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[n] = __float2bfloat16_rn(y);
+    else reinterpret_cast<float*>(p.out)[n] = y;
+  }
+}
+
+template <int DT>
+static int launch_row(const SkLinear& p, cudaStream_t st) {
+  const bool vec = (uintptr_t)p.x % (4 * sizeof(typename In<DT>::T)) == 0;
+  const unsigned grid = (unsigned)((p.N + 15) / 16);
+  // eight warps share a row block's K while there are few of them
+  if (grid <= 2u * (unsigned)device_sm_count()) {
+    if (vec) sk_row_kernel<DT, true, 8><<<grid, 256, 0, st>>>(p);
+    else sk_row_kernel<DT, false, 8><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (vec) sk_row_kernel<DT, true, 4><<<grid, 128, 0, st>>>(p);
+    else sk_row_kernel<DT, false, 4><<<grid, 128, 0, st>>>(p);
+  }
+  return check_launch("sk_row_kernel");
+}
+
+// Cold L2, against the tcgen05 kernel: 16 x 1408 x 2816 12.3 and 20.5 us, 48 x
+// 2112 x 2816 18.4 and 20.5, but 32 x 8192 x 8192 67.6 and 36.9 (every CTA
+// reads all of the codes), 16 x 8192 x 8192 36.9 and 36.9, 64 x 2816 x 704 18.5
+// and 14.3.
+bool fb_linear_skinny_takes(int64_t M, int64_t N, int64_t K) {
+  return M <= 16 || (M <= 48 && N * K <= (1 << 23));
+}
 
 template <int DT>
 static int launch_quant(const SkLinear& p, cudaStream_t st) {
@@ -206,22 +327,37 @@ int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uin
   p.out = out;
   p.out_dt = out_dt;
   p.ldc = ldc;
+  if (x && M == 1) {
+    if (dtype == AEOQ_BF16) return launch_row<AEOQ_BF16>(p, st);
+    if (dtype == AEOQ_F16) return launch_row<AEOQ_F16>(p, st);
+    return launch_row<AEOQ_F32>(p, st);
+  }
   if (x && M <= kFbSkinnyQuant) {
     if (dtype == AEOQ_BF16) return launch_quant<AEOQ_BF16>(p, st);
     if (dtype == AEOQ_F16) return launch_quant<AEOQ_F16>(p, st);
     return launch_quant<AEOQ_F32>(p, st);
   }
   if (x) {
-    const int rc = fb_quantize_rows(x, dtype, M, K, ldx, nullptr, nullptr, q, K, qs, st);
+    const int rc = fb_quantize_rows(x, dtype, M, K, ldx, q, K, qs, st);
     if (rc) return rc;
   }
   p.q = q;
   p.qs = qs;
-  const unsigned grid = (unsigned)((N + 15) / 16);
-  if (M <= 8) sk_linear_kernel<AEOQ_BF16, false, true, 1><<<grid, kSkThreads, 0, st>>>(p);
-  else if (M <= 16) sk_linear_kernel<AEOQ_BF16, false, true, 2><<<grid, kSkThreads, 0, st>>>(p);
-  else if (M <= 32) sk_linear_kernel<AEOQ_BF16, false, true, 4><<<grid, kSkThreads, 0, st>>>(p);
-  else sk_linear_kernel<AEOQ_BF16, false, true, 8><<<grid, kSkThreads, 0, st>>>(p);
+  // With the quantizer just before it, the kernel starts while that runs and
+  // requests its weights meanwhile.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((N + 15) / 16));
+  cfg.blockDim = dim3(kSkThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = x ? 1 : 0;
+  if (M <= 8) cudaLaunchKernelEx(&cfg, sk_linear_kernel<AEOQ_BF16, false, true, 1>, p);
+  else if (M <= 16) cudaLaunchKernelEx(&cfg, sk_linear_kernel<AEOQ_BF16, false, true, 2>, p);
+  else if (M <= 32) cudaLaunchKernelEx(&cfg, sk_linear_kernel<AEOQ_BF16, false, true, 4>, p);
+  else cudaLaunchKernelEx(&cfg, sk_linear_kernel<AEOQ_BF16, false, true, 8>, p);
   return check_launch("sk_linear_kernel");
 }
 
@@ -237,27 +373,6 @@ struct SkExperts {
   float* h;                 // (pairs, I)
   __nv_bfloat16* out;       // (T, H)
 };
-
-// One warp's codes of a row of one block, four values per lane: written to
-// `codes` (128 bytes) in shared memory, the scale returned to every lane.
-__device__ __forceinline__ float sk_quantize_warp(const float (&v)[4], uint8_t* codes) {
-  const int lane = threadIdx.x & 31;
-  uint32_t key = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) key = max(key, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  key = __reduce_max_sync(0xFFFFFFFFu, key);
-  const float2 s = fb_scales(__uint_as_float(key));
-  reinterpret_cast<uint32_t*>(codes)[lane] = fb_codes4(v[0] * s.x, v[1] * s.x, v[2] * s.x, v[3] * s.x);
-  return s.y;
-}
-
-// A lane's piece of a row's codes in shared memory, for every column alike.
-__device__ __forceinline__ void sk_codes(const uint8_t* codes, uint32_t (&c)[8]) {
-  const uint4* q = reinterpret_cast<const uint4*>(codes + 32 * (threadIdx.x & 3));
-  const uint4 a = q[0], b = q[1];
-  c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
-  c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
-}
 
 // h = act(gate x) * up x of one pair (token, slot). CTA (x, y): features 8 x ..
 // 8 x + 7 (their gate rows are the MMA's rows 0-7, their up rows 8-15) of pair
