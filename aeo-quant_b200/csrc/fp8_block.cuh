@@ -99,12 +99,35 @@ enum FbActivation : int { kFbGeluTanh = 0, kFbSilu = 1 };
 
 // gelu(x, tanh form) = x * sigmoid(2 z), z = sqrt(2/pi) (x + 0.044715 x^3),
 // since 1 + tanh(z) = 2 sigmoid(2 z); silu(x) = x * sigmoid(x). Written so,
-// neither cancels for negative x. __expf's relative error grows with its
-// argument (about 2^-22 + |arg| 2^-24); where |arg| is large the result is 0
-// or x to within f32.
-__device__ __forceinline__ float fb_act(int act, float x) {
-  const float a = act == kFbSilu ? x : 1.5957691216057308f * (x + 0.044715f * (x * x * x));
-  return __fdividef(x, 1.0f + __expf(-a));
+// neither cancels for negative x. Both are x / (1 + 2^(-x (c0 + c1 x^2))) with
+// constants of their own, log2 e among them. The approximate 2^x and 1/x are
+// within 2^-22 each, and an exponent a brings |a| 2^-24; where that is large
+// the result is 0 or x to within f32. (The library's __expf and __fdividef
+// take care of denormals too: the epilogue of 4096 tokens' gate_up 66 us
+// longer.)
+__device__ __forceinline__ float2 fb_act_of(int act) {
+  return act == kFbSilu ? make_float2(-1.4426950408889634f, 0.0f)
+                        : make_float2(-2.302208198f, -0.1029432396f);   // -2 sqrt(2/pi) log2 e, times 0.044715
+}
+__device__ __forceinline__ float fb_act(float2 c, float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * fmaf(c.y, fminf(x * x, 1e30f), c.x)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return x * r;
+}
+
+// Two at once with one reciprocal, 1/a = b/(ab): the two approximations per
+// value are what the epilogues wait for (16 per SM and cycle). The exponents
+// are held at 60 so that the product stays finite: where x / (1 + 2^60) is
+// returned, the exact value is as good as 0 beside any other.
+__device__ __forceinline__ float2 fb_act2(float2 c, float x, float y) {
+  float a, b, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fminf(x * fmaf(c.y, fminf(x * x, 1e30f), c.x), 60.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fminf(y * fmaf(c.y, fminf(y * y, 1e30f), c.x), 60.0f)));
+  a += 1.0f;
+  b += 1.0f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return make_float2(x * (r * b), y * (r * a));
 }
 
 // Few rows of a: the weights are streamed through mma.sync (fp8_block_skinny.cu).

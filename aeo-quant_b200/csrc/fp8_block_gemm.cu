@@ -224,11 +224,14 @@ __device__ __forceinline__ void fb_glu_half(const FbParams& p, const FbTile& cur
                                             float (&acc)[128], int row, int half, bool alive) {
   const int64_t n0 = cur.n0 + 64 * half;
   const int n_ok = (int)min((int64_t)64, p.I - n0);
+  const float2 ac = fb_act_of(p.act);
   uint32_t key = 0;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    acc[i] = i < n_ok ? fb_act(p.act, acc[i]) * acc[64 + i] : 0.0f;
-    key = max(key, __float_as_uint(acc[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 64; i += 2) {
+    const float2 v = fb_act2(ac, acc[i], acc[i + 1]);
+    acc[i] = i < n_ok ? v.x * acc[64 + i] : 0.0f;
+    acc[i + 1] = i < n_ok ? v.y * acc[65 + i] : 0.0f;      // n_ok is even
+    key = max(key, max(__float_as_uint(acc[i]) & 0x7FFFFFFFu, __float_as_uint(acc[i + 1]) & 0x7FFFFFFFu));
   }
   if (both) {
     amax[half][row] = __uint_as_float(key);
@@ -699,9 +702,10 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
       } else {
         // the block of 128 features of a token is this tile's 128 lanes
         const bool in = ti.n0 + f < p.I;
+        const float2 ac = fb_act_of(p.act);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          acc[0][j] = in ? fb_act(p.act, acc[0][j]) * acc[1][j] : 0.0f;
+          acc[0][j] = in ? fb_act(ac, acc[0][j]) * acc[1][j] : 0.0f;
           const uint32_t k = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(acc[0][j]) & 0x7FFFFFFFu);
           if (lane == j) sh->amax[half][q][j] = k;
         }

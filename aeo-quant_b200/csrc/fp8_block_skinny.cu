@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(32 * kSkGuWarps, 5) sk_gate_up_kernel(const Sk
       gate += part[w][threadIdx.x];
       up += part[w][threadIdx.x + 8];
     }
-    p.h[(int64_t)y * p.I + f0 + threadIdx.x] = fb_act(p.act, gate) * up;
+    p.h[(int64_t)y * p.I + f0 + threadIdx.x] = fb_act(fb_act_of(p.act), gate) * up;
   }
 }
 
