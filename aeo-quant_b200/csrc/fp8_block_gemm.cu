@@ -356,8 +356,9 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         __syncwarp();
         continue;
       }
-      if (!sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72) ||
-          !sm100::mbar_wait(&sh->full[s], ph, p.err, 73))
+      // (the accumulator last: it is what comes last)
+      if (!sm100::mbar_wait(&sh->full[s], ph, p.err, 73) ||
+          !sm100::mbar_wait(&sh->acc_empty[b], bph ^ 1, p.err, 72))
         break;
       sm100::tc_fence_after();
       if (leader) {
@@ -366,8 +367,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         for (int j = 0; j < 4; ++j)
           sm100::tc_mma_f8(tmem + b * BN, sm100::sdesc_k_sw128(sa + 32 * j), sm100::sdesc_k_sw128(sb + 32 * j), idesc,
                            j ? 1u : 0u);
-        sm100::tc_commit(&sh->empty[s]);
         sm100::tc_commit(&sh->acc_full[b]);
+        sm100::tc_commit(&sh->empty[s]);
       }
       __syncwarp();
     }

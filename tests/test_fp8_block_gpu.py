@@ -123,7 +123,8 @@ def test_linear_sizes(M, N, K):
 
 
 @pytest.mark.parametrize("M,N,K", [(4096, 1408, 2816), (5000, 257, 144), (1500, 4000, 1040), (40, 30000, 256),
-                                   (1, 40000, 512), (20000, 384, 128)])
+                                   (1, 40000, 512), (20000, 384, 128), (40, 8192, 2048), (8, 6000, 4096),
+                                   (2100, 1408, 272), (1, 1000, 16400)])
 def test_linear_large(M, N, K):
     w, s = weights(N + K, 1, N, K)
     check_linear(randn(M, M, K), w[0], s[0])
@@ -243,7 +244,10 @@ def test_experts_sizes(T, E, k, H, I, act):
     check_experts(randn(T, T, H), *routing(T, T, E, k), gu, gs, dw, ds, act)
 
 
-@pytest.mark.parametrize("T,E,k,H,I", [(1500, 8, 2, 512, 256), (300, 128, 8, 256, 128), (700, 3, 3, 1040, 448)])
+@pytest.mark.parametrize("T,E,k,H,I", [(1500, 8, 2, 512, 256), (300, 128, 8, 256, 128), (700, 3, 3, 1040, 448),
+                                       (900, 16, 8, 272, 192), (600, 128, 8, 144, 64), (70, 1024, 4, 64, 64),
+                                       (2000, 1024, 3, 64, 64), (5000, 4, 1, 128, 64), (30, 4, 4, 16, 64),
+                                       (4097, 32, 1, 16, 128)])
 def test_experts_many_tokens(T, E, k, H, I):
     gu, gs = weights(E + H, E, 2 * I, H)
     dw, ds = weights(E + I, E, H, I)
