@@ -1,4 +1,5 @@
-// Expert choice from router logits, one warp per token.
+// Expert choice from router logits, one warp per token (many rows of 16-bit
+// logits alone: one thread, see there).
 //
 //   s = softmax(l) or 1 / (1 + exp(-l))            score of each expert
 //   c = s + bias, and -inf where l = -inf          what the choice goes by
@@ -446,7 +447,12 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
 // the warp above takes some 800. The rows are staged through shared memory,
 // read with whole lines.
 constexpr int kRouteRowThreads = 128;
-constexpr int kRouteRowsFrom = 4096;     // rows: see below
+// From how many rows, of bf16 and k = 8 (us, the warp kernel / this one):
+// 64 experts 2048 rows 6.2 / 6.2, 8192 rows 10.3 / 6.2; 128 experts 2048 rows
+// 6.2 / 8.3, 4096 rows 8.3 / 8.3, 65536 rows 51 / 17; 256 experts 4096 rows
+// 10.0 / 12.5, 8192 rows 14.4 / 12.5; 512 experts 8192 rows 20.9 / 20.6, 16384
+// rows 37 / 21. With fewer rows its threads, one per row, do not fill the SMs.
+constexpr int64_t kRouteRowsFrom = 4096, kRouteRowsPerExpert = 32;
 
 __device__ __forceinline__ void key_pair(uint32_t& a, uint32_t& b) {
   const uint32_t t = max(a, b);
@@ -593,7 +599,7 @@ static int dispatch_route(RouteParams p, cudaStream_t st) {
   if constexpr (DT != AEOQ_F32) {
     const bool logits_alone = !p.bias && p.n_group == 1;
     if (logits_alone && p.k <= 8 && p.E >= 8 && p.E <= 512 && p.E % 8 == 0 && (uintptr_t)p.logits % 16 == 0 &&
-        (p.ld * 2) % 16 == 0 && p.T >= kRouteRowsFrom)
+        (p.ld * 2) % 16 == 0 && p.T >= std::max(kRouteRowsFrom, kRouteRowsPerExpert * p.E))
       return launch_route_rows<DT>(p, st);
   }
   switch (per) {

@@ -75,6 +75,7 @@ def test_many_rows_with_bias():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k", [(4096, 128, 8), (5003, 256, 3), (4100, 8, 8), (4097, 512, 1), (4099, 136, 5),
+                                   (8193, 256, 3), (16390, 512, 1), (4359, 136, 5),
                                    (4096, 520, 4), (4098, 130, 8)])
 def test_many_16_bit_rows(dtype, T, E, k):
     """The row counts at which one thread takes a row: ties, masks, NaN and
