@@ -570,15 +570,10 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
   const uint32_t tmem = sh->tmem_base;
   const int total = sh->tile_off[p.E] * p.tiles_n, KB = p.KB;
   constexpr int kWide = EPI == kFbGlu ? 128 : 256;      // output columns of a tile
-  // the last column of tiles may read half of a tile's rows of w or fewer:
-  // those go last (16 tokens, 128 experts, I = 704: the layer 91 -> 88 us)
-  const int last = (int)((EPI == kFbGlu ? p.I : p.N) - (int64_t)(p.tiles_n - 1) * kWide);
-  const bool half_last = last <= kWide / 2;
   auto tile = [&](int t) {
     FbTile r;
-    const int2 at = fb_place(t, sh->tile_off[p.E], p.tiles_n, half_last);
-    const int ct = at.x;
-    r.n0 = (int64_t)at.y * kWide;
+    const int ct = t / p.tiles_n;
+    r.n0 = (int64_t)(t - ct * p.tiles_n) * kWide;
     int lo = 0, hi = p.E;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
