@@ -125,6 +125,16 @@ def load_gemma4_fp8_block(model_id_or_path, **from_pretrained_kwargs):
     return _install_fused_routers(model)
 
 
+def _activation_name(experts) -> str:
+    """The config name of an expert module's activation."""
+    from transformers.activations import ACT2FN
+    for name in ("gelu_pytorch_tanh", "silu"):
+        if type(experts.act_fn) is type(ACT2FN[name]):
+            return name
+    raise ValueError(f"the experts' activation {type(experts.act_fn).__name__} is not supported by the fused kernels "
+                     "(gelu_pytorch_tanh or silu)")
+
+
 @torch.no_grad()
 def quantize_experts_to_fp8_block(model):
     """Replace every bf16 ``Gemma4TextExperts`` in ``model`` by a
@@ -138,10 +148,12 @@ def quantize_experts_to_fp8_block(model):
     for _, mod in model.named_modules():
         for child_name, child in mod.named_children():
             if type(child) is modeling_gemma4.Gemma4TextExperts:
-                targets.append((mod, child_name, child))
-    for parent, child_name, old in targets:
+                targets.append((mod, child_name, child, _activation_name(child)))
+    for parent, child_name, old, activation in targets:
+        shape = _ExpertShape(old)
+        shape.hidden_activation = activation
         with torch.device("meta"):
-            new = Gemma4TextExpertsFP8Block(_ExpertShape(old))
+            new = Gemma4TextExpertsFP8Block(shape)
         for proj in ("gate_up_proj", "down_proj"):
             q, scale = quantize_3d_to_fp8_block(getattr(old, proj).detach())
             setattr(new, proj, torch.nn.Parameter(q, requires_grad=False))

@@ -53,6 +53,30 @@ def test_class_swap_and_dispatch_cpu(monkeypatch):
     assert seen == [("p", {"device_map": "cpu"})]
 
 
+@pytest.mark.parametrize("act", ["gelu_pytorch_tanh", "silu", "relu"])
+def test_conversion_keeps_the_activation_cpu(monkeypatch, act):
+    """Experts are converted with the activation they have, or refused before
+    any of them is replaced."""
+    from transformers.models.gemma4.modeling_gemma4 import Gemma4TextExperts
+    from aeo_quant_b200.bridges.gemma4 import loader
+    from aeo_quant_b200.bridges.gemma4.modeling_fp8_block import Gemma4TextExpertsFP8Block
+    from aeo_quant_b200.gpu import quant
+    monkeypatch.setattr(quant, "quantize_3d_to_fp8_block", lambda w: (
+        w.to(F8), torch.ones(w.shape[0], -(-w.shape[1] // 128), -(-w.shape[2] // 128))))
+    model = nn.Module()
+    model.experts = Gemma4TextExperts(config(act=act))
+    for p in model.experts.parameters():
+        nn.init.zeros_(p)
+    if act == "relu":
+        with pytest.raises(ValueError, match="not supported"):
+            loader.quantize_experts_to_fp8_block(model)
+        assert type(model.experts) is Gemma4TextExperts
+        return
+    assert loader.quantize_experts_to_fp8_block(model) == 1
+    assert type(model.experts) is Gemma4TextExpertsFP8Block
+    assert model.experts.activation == act and model.experts.gate_up_proj_scale.shape == (8, 3, 2)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape,N,K,bias", [((7,), 2112, 2816, False), ((2, 5), 200, 144, True), ((1,), 96, 64, True),
                                             ((3, 50), 384, 256, False)])
