@@ -488,7 +488,10 @@ static int launch_gemm(const uint8_t* a, int64_t a_rows, const uint8_t* w, FbPar
   rc = make_tmap_bytes(&tw, w, p.E * p.N, p.K, p.K, 128, EPI == kFbGlu ? BN / 4 : BN, true);
   if (rc) return rc;
   to = ta;
-  p.out_tma = EPI == kFbStore && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0;
+  // (a column's byte is a 32-bit coordinate of the store, and a row that does
+  // not end on 16 bytes was written beyond its last column: N = 127, ldc = 136)
+  p.out_tma = EPI == kFbStore && p.out_dt == AEOQ_BF16 && p.ldc % 8 == 0 && (uintptr_t)p.out % 16 == 0 &&
+              p.N % 8 == 0 && p.N <= (1 << 30);
   if (p.out_tma) {
     rc = make_tmap_bytes(&to, p.out, p.M, p.N * 2, p.ldc * 2, 128, 128, true);
     if (rc) return rc;

@@ -312,3 +312,110 @@ def test_experts_strides_stream_graph():
         bi.copy_(i)
         graph.replay()
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------- C entry, sizes, streams
+@pytest.mark.parametrize("out_dt", [0, 2])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 256), (5, 200, 144), (40, 130, 256), (300, 400, 256), (257, 127, 400)])
+@pytest.mark.parametrize("pad,shift", [(8, 0), (3, 0), (8, 1)])
+def test_linear_into_a_larger_output(M, N, K, out_dt, pad, shift):
+    """Rows of a larger output, aligned for wide stores or not: what lies
+    between and behind the product's values stays as it was."""
+    from aeo_quant_b200 import _capi as A
+    from aeo_quant_b200.gpu.fp8_block_matmul import fp8_block_linear
+    dt = torch.bfloat16 if out_dt == 0 else torch.float32
+    x = randn(21, M, K)
+    w, s = weights(22, 1, N, K)
+    ldc = (N + 7) // 8 * 8 + pad
+    buf = torch.full(((M + 2) * ldc + shift,), 7.0, dtype=dt, device="cuda")
+    out = buf[shift:].view(M + 2, ldc)
+    n = A.load().aeoq_fp8_block_linear_workspace_size(M, N, K)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    A.check(A.load().aeoq_fp8_block_linear(x.data_ptr(), A.dtype_code(x.dtype), K, M, w[0].data_ptr(),
+                                           s[0].data_ptr(), N, K, None, out.data_ptr(), out_dt, ldc, ws.data_ptr(), n,
+                                           A.err_ptr(0), A.raw_stream(torch.cuda.current_device())))
+    assert torch.equal(out[:M, :N], fp8_block_linear(x, w[0], s[0], out_dtype=dt))
+    assert bool((out[:M, N:] == 7).all()) and bool((out[M:] == 7).all()) and bool((buf[:shift] == 7).all())
+
+
+def test_rows_past_32_bit_offsets():
+    """Input rows that start past 2^31 elements."""
+    from aeo_quant_b200.gpu.fp8_block_matmul import fp8_block_linear
+    from aeo_quant_b200.gpu.quant import quantize_fp8_activation_blocks
+    w, s = weights(23, 1, 200, 512)
+    for M, ld in ((4, 1 << 30), (20, 1 << 27), (300, 1 << 23)):
+        x = torch.empty((M - 1) * ld + 512, dtype=torch.bfloat16, device="cuda").as_strided((M, 512), (ld, 1))
+        x.copy_(randn(24, M, 512))
+        near = x.contiguous()
+        for a, b in zip(quantize_fp8_activation_blocks(x), quantize_fp8_activation_blocks(near)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(fp8_block_linear(x, w[0], s[0]), fp8_block_linear(near, w[0], s[0]))
+        del x
+
+
+def test_experts_past_32_bit_offsets():
+    """Experts whose weights start past 2^31 bytes, and tokens whose experts'
+    outputs start past 2^31 values: the same bits as from a small layer."""
+    from aeo_quant_b200.bridges.gemma4.moe_ops import fp8_block_experts
+    E, H, I = 9, 16384, 8192
+    g = gen(25)
+
+    def codes(*shape):
+        return torch.randint(0, 0x60, shape, dtype=torch.uint8, device="cuda", generator=g).view(F8)
+
+    def scales(E, n, k):
+        return torch.rand(E, -(-n // 128), -(-k // 128), device="cuda", generator=g) * 1e-4
+    gu, gs, dw, ds = codes(E, 2 * I, H), scales(E, 2 * I, H), codes(E, H, I), scales(E, H, I)
+    for T in (1, 36, 250):          # each of the three forms: 2 T pairs on 9 or 2 experts
+        x = randn(26, T, H)
+        ids = torch.tensor([[E - 1, E - 2]], device="cuda").repeat(T, 1)
+        w = torch.rand(T, 2, device="cuda", generator=g)
+        big = fp8_block_experts(x, ids, w, gu, gs, dw, ds, activation="silu")
+        small = fp8_block_experts(x, ids - (E - 2), w, *(t[E - 2:] for t in (gu, gs, dw, ds)), activation="silu")
+        assert torch.equal(big, small) and bool(torch.isfinite(big).all())
+    del gu, dw
+    I, T, n = 64, 70000, 100
+    gu, gs, dw, ds = codes(2, 2 * I, H), scales(2, 2 * I, H), codes(2, H, I), scales(2, H, I)
+    x = randn(27, T, H)
+    ids = torch.tensor([[0, 1]], device="cuda").repeat(T, 1)
+    w = torch.rand(T, 2, device="cuda", generator=g)
+    big = fp8_block_experts(x, ids, w, gu, gs, dw, ds)
+    assert torch.equal(big[-n:], fp8_block_experts(x[-n:], ids[-n:], w[-n:], gu, gs, dw, ds))
+
+
+def test_experts_on_two_streams_at_once():
+    """Calls that overlap, eager and as two captured graphs, share nothing."""
+    from aeo_quant_b200.bridges.gemma4.moe_ops import fp8_block_experts
+    E, k, H, I = 16, 4, 512, 128
+    gu, gs = weights(28, E, 2 * I, H)
+    dw, ds = weights(29, E, H, I)
+    jobs = []
+    for i, T in enumerate((3, 40, 700, 2, 55, 900)):
+        ids, w = routing(30 + i, T, E, k)
+        x = randn(40 + i, T, H)
+        jobs.append((x, ids, w, fp8_block_experts(x, ids, w, gu, gs, dw, ds)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(5):
+        for j, (x, ids, w, _) in enumerate(jobs):
+            with torch.cuda.stream(streams[j]):
+                got[j].append(fp8_block_experts(x, ids, w, gu, gs, dw, ds))
+    torch.cuda.synchronize()
+    for j, (_, _, _, want) in enumerate(jobs):
+        assert all(torch.equal(want, y) for y in got[j])
+    graphs = []
+    for x, ids, w, _ in jobs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = fp8_block_experts(x, ids, w, gu, gs, dw, ds)
+        graphs.append((graph, y))
+    for _, y in graphs:
+        y.zero_()
+    torch.cuda.synchronize()
+    for st, (graph, _) in zip(streams, graphs):
+        with torch.cuda.stream(st):
+            graph.replay()
+    torch.cuda.synchronize()
+    for (_, y), (_, _, _, want) in zip(graphs, jobs):
+        assert torch.equal(y, want)
