@@ -378,8 +378,8 @@ def fp8_block_experts(hidden, top_k_index, top_k_weights, gu, gu_scale, dw, dw_s
     ``hidden`` (T, H) bfloat16, quantized per 128 values of a row, as the
     experts' intermediate rows are; ``gu`` (E, 2I, H) with ``gu_scale`` (E,
     ceil(2I/128), ceil(H/128)), ``dw`` (E, H, I) with ``dw_scale`` (E,
-    ceil(H/128), ceil(I/128)); an id outside [0, E) adds nothing. Sums are
-    f32; the output is bfloat16. H must be a multiple of 16, I of 64."""
+    ceil(H/128), ceil(I/128)); an id outside [0, E) adds nothing. All sums
+    are f32, rounded once to the bfloat16 output. H must be a multiple of 16, I of 64."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
     if hidden.ndim != 2 or hidden.dtype != torch.bfloat16:

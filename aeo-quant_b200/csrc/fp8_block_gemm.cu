@@ -178,8 +178,9 @@ __device__ __forceinline__ void fb_store_tile(const FbParams& p, const CUtensorM
   }
 }
 
-// The other tiles (behind a short one lie another expert's rows; f32; rows
-// that are not 16-byte aligned), rows and columns left out one by one: each
+// f32 (the experts' outputs among them: behind a short tile lie another
+// expert's rows) and rows that are not 16-byte aligned, rows and columns left
+// out one by one: each
 // warp turns its 32 rows around in 4 KB of shared memory, 128 bytes of a row
 // at a time, so that a store instruction writes four whole lines.
 template <class T, int kCols>
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         uint8_t* box = base + L::kStages * L::kStage + half * (128 * kCols * 2);
         if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-        if (p.out_tma && (cur.rows == 128 || !p.grp_off)) fb_store_tile(p, tmO, cur, box, acc, row, half, alive);
+        if (p.out_tma) fb_store_tile(p, tmO, cur, box, acc, row, half, alive);
         else if (p.out_dt == AEOQ_BF16) fb_store_rows<__nv_bfloat16>(p, cur, box + q * 4096, acc, q, half, alive);
         else fb_store_rows<float>(p, cur, box + q * 4096, acc, q, half, alive);
       } else {
@@ -704,14 +705,14 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
         }
       }
       if constexpr (EPI == kFbStore) {
-        // 32 lanes store 64 consecutive bytes of a token's row
-        __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + (ti.row0 + tok0) * p.ldc + ti.n0 + f;
+        // 32 lanes store 128 consecutive bytes of a token's row
+        float* d = reinterpret_cast<float*>(p.out) + (ti.row0 + tok0) * p.ldc + ti.n0 + f;
         if (!alive) continue;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           if (j >= n_tok) break;
-          if (ti.n0 + f < p.N) d[j * p.ldc] = __float2bfloat16_rn(acc[0][j]);
-          if (ti.n0 + 128 + f < p.N) d[j * p.ldc + 128] = __float2bfloat16_rn(acc[1][j]);
+          if (ti.n0 + f < p.N) d[j * p.ldc] = acc[0][j];
+          if (ti.n0 + 128 + f < p.N) d[j * p.ldc + 128] = acc[1][j];
         }
       } else {
         // the block of 128 features of a token is this tile's 128 lanes
@@ -876,11 +877,14 @@ static int launch_sort(const void* ids, int ids_dt, int64_t n_pairs, int k, int 
 }
 
 // out[t] = sum over slots j, in order, of weights[t][j] * y[pair_row[t][j]], in
-// f32, rounded once; a slot without an expert adds nothing. The loads of
-// kFbCombineSlots slots are in flight together (4096 tokens, top-8, H = 2816:
-// one 41 us, 4 38 us, which is 5.4 TB/s, 8 47 us).
+// f32, rounded once; a slot without an expert adds nothing. y is f32 as well:
+// held in bf16, each expert's output would be rounded too, 1.41 times the
+// error of the one rounding, and where the experts' outputs cancel more (at 4096
+// tokens, top-8, H = 2816 that would take 38 us here for 68, and 155 for 192
+// in the GEMM that writes it). The loads of kFbCombineSlots slots are in flight
+// together (same size: one 69 us, 2 and 4 68 us, which is 6.1 TB/s, 8 102 us).
 constexpr int kFbCombineSlots = 4;
-__global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __restrict__ y,
+__global__ void __launch_bounds__(256) fb_combine_kernel(const float* __restrict__ y,
                                                          const int* __restrict__ pair_row,
                                                          const float* __restrict__ weights, int64_t T, int k,
                                                          int64_t H, __nv_bfloat16* __restrict__ out) {
@@ -891,7 +895,7 @@ __global__ void __launch_bounds__(256) fb_combine_kernel(const __nv_bfloat16* __
     for (int j0 = 0; j0 < k; j0 += kFbCombineSlots) {
       int r[kFbCombineSlots];
       float w[kFbCombineSlots];
-      FbEight<AEOQ_BF16> v[kFbCombineSlots];
+      FbEight<AEOQ_F32> v[kFbCombineSlots];
 #pragma unroll
       for (int j = 0; j < kFbCombineSlots; ++j) {
         r[j] = j0 + j < k ? __ldg(pair_row + t * k + j0 + j) : -1;
@@ -944,7 +948,7 @@ struct FbExpertsWs {
     xs = take(4 * rows * fb_blocks(H));
     hq = take(P * I);
     hs = take(4 * P * fb_blocks(I));
-    y = take(2 * P * H);
+    y = take(4 * P * H);
     bytes = o;
   }
 };
@@ -1097,14 +1101,14 @@ extern "C" int aeoq_moe_fp8_block_forward(const void* hidden, int64_t T, const v
   d.tile_off = ints(l.tile_off);
   d.tiles_n = (int)((H + 255) / 256);
   d.out = ws + l.y;
-  d.out_dt = AEOQ_BF16;
+  d.out_dt = AEOQ_F32;
   d.ldc = H;
   d.err = err_word;
   rc = few ? launch_few<kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st)
            : launch_gemm<256, kFbStore>(ws + l.hq, P, down, d, max_tiles * d.tiles_n, st);
   if (rc) return rc;
   const unsigned blocks = (unsigned)std::min<int64_t>((T * (H / 8) + 255) / 256, (int64_t)device_sm_count() * 16);
-  fb_combine_kernel<<<blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(ws + l.y), ints(l.pair_row),
+  fb_combine_kernel<<<blocks, 256, 0, st>>>(floats(l.y), ints(l.pair_row),
                                             top_k_weights, T, (int)k, H, reinterpret_cast<__nv_bfloat16*>(out));
   return check_launch("fb_combine_kernel");
 }

@@ -552,8 +552,8 @@ AEOQ_API int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int64_
  * outside [0, num_experts) adds nothing; top_k_weights (T, k) f32; gate_up
  * (E, 2I, H) and down (E, H, I) e4m3; their scales (E, ceil(2I/128),
  * ceil(H/128)) and (E, ceil(H/128), ceil(I/128)) f32; out (T, H) bf16.
- * H % 16 == 0, I % 64 == 0, k <= 32, E <= 1024. Sums are f32, the experts'
- * outputs are held in bf16 before the weighted sum.
+ * H % 16 == 0, I % 64 == 0, k <= 32, E <= 1024. All sums are f32, the
+ * weighted one over a token's experts too; out is rounded once.
  * ------------------------------------------------------------------------ */
 AEOQ_API size_t aeoq_moe_fp8_block_workspace_size(int64_t T, int64_t top_k, int64_t num_experts, int64_t hidden,
                                                   int64_t inter);
