@@ -109,25 +109,38 @@ __device__ __forceinline__ float2 fb_act_of(int act) {
   return act == kFbSilu ? make_float2(-1.4426950408889634f, 0.0f)
                         : make_float2(-2.302208198f, -0.1029432396f);   // -2 sqrt(2/pi) log2 e, times 0.044715
 }
+// The exponent of that 2^x: the lower x, the larger.
+__device__ __forceinline__ float fb_act_exponent(float2 c, float x) {
+  return x * fmaf(c.y, fminf(x * x, 1e30f), c.x);
+}
+
 __device__ __forceinline__ float fb_act(float2 c, float x) {
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * fmaf(c.y, fminf(x * x, 1e30f), c.x)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fb_act_exponent(c, x)));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return x * r;
 }
 
 // Two at once with one reciprocal, 1/a = b/(ab): the two approximations per
-// value are what the epilogues wait for (16 per SM and cycle). The exponents
-// are held at 60 so that the product stays finite: where x / (1 + 2^60) is
-// returned, the exact value is as good as 0 beside any other.
+// value are what the epilogues wait for (16 per SM and cycle). a = 1 + 2^x is
+// held times 2^-63, so that the product of two of up to 2^126 each stays
+// finite and its reciprocal normal; from there on 1/a is 0, as the reciprocal
+// above makes it. (Gates that far below 0 still count where a whole block of
+// 128 values is tiny: their largest sets the scale. With a cut at 2^60
+// such a block came out up to 2^66 times too large; that took 206 us for the
+// gate_up of 4096 tokens, this 208, and a branch to two reciprocals, which some
+// pair of most warps needs, 231.)
 __device__ __forceinline__ float2 fb_act2(float2 c, float x, float y) {
+  constexpr float kMost = 126.0f, kDown = 0x1p-63f;
+  const float u = fb_act_exponent(c, x), v = fb_act_exponent(c, y);
   float a, b, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fminf(x * fmaf(c.y, fminf(x * x, 1e30f), c.x), 60.0f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fminf(y * fmaf(c.y, fminf(y * y, 1e30f), c.x), 60.0f)));
-  a += 1.0f;
-  b += 1.0f;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fminf(u, kMost)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fminf(v, kMost)));
+  a = fmaf(a, kDown, kDown);
+  b = fmaf(b, kDown, kDown);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-  return make_float2(x * (r * b), y * (r * a));
+  const float p = u > kMost ? 0.0f : r * b * kDown, q = v > kMost ? 0.0f : r * a * kDown;
+  return make_float2(x * p, y * q);
 }
 
 // Few rows of a: the weights are streamed through mma.sync (fp8_block_skinny.cu).

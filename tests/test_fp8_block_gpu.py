@@ -1,5 +1,7 @@
 """Block-scaled FP8 kernels against the 64-bit oracle: codes and scales bit for
 bit, products within the oracle's bounds."""
+import math
+
 import pytest
 import torch
 
@@ -441,3 +443,43 @@ def test_experts_round_once(T, E, k, H, I):
     ref, _ = O.experts(x.double(), ids, w.double(), gu.double(), gs.double(), dw.double(), ds.double(), "silu")
     once = (ref.bfloat16().double() - ref).norm()
     assert float((y.double() - ref).norm()) <= 1.2 * float(once)
+
+
+# ------------------------------------------------------ strongly negative gates
+@pytest.mark.parametrize("T,E", [(1, 2), (100, 4), (300, 2)])
+@pytest.mark.parametrize("act,gain", [("gelu_pytorch_tanh", 1.25), ("silu", 6.0), ("silu", 2.0 ** 60),
+                                      ("gelu_pytorch_tanh", 2.0 ** 60)])
+@pytest.mark.parametrize("I", [64, 192])
+def test_experts_strongly_negative_gates(T, E, act, gain, I):
+    """Where all of a block's gates are strongly negative, their tiny values
+    set the block's scale and are kept with full codes. The operands are
+    chosen so that gates and ups are exact: one value per row of x whose code
+    and scale are exact (7 = 448 / 2^6), one product per sum."""
+    from aeo_quant_b200.bridges.gemma4.moe_ops import fp8_block_experts
+    H = 128
+    x = torch.zeros(T, H, device="cuda", dtype=torch.bfloat16)
+    x[:, 0] = 7.0
+    gu = torch.zeros(E, 2 * I, H, device="cuda")
+    gu[:, :I, 0] = -(1 + torch.randint(0, 7, (E, I), generator=gen(I), device="cuda") / 8)     # -1 ... -1.75
+    gu[:, I:, 0] = (1 + torch.randint(0, 8, (E, I), generator=gen(I + 1), device="cuda") / 8)
+    gs = torch.ones(E, -(-2 * I // 128), 1, device="cuda")
+    gs[:, :I // 128] = gain
+    if I % 128:
+        gs[:, I // 128] = gain            # this block holds gates and ups
+    dw = torch.zeros(E, H, I, device="cuda")
+    dw[:, torch.arange(H), torch.arange(H) % I] = 1.0
+    ds = torch.ones(E, 1, -(-I // 128), device="cuda")
+    ids = torch.arange(T, device="cuda")[:, None] % E
+    w = torch.ones(T, 1, device="cuda")
+    y = fp8_block_experts(x, ids, w, gu.to(F8), gs, dw.to(F8), ds, activation=act).double()
+    xd = O.value_rows(*O.quantize_rows(x.double()))
+    full = torch.einsum("th,enh->ten", xd, O.value_blocks(gu.double(), gs.double()))
+    g, u = full[torch.arange(T), ids[:, 0]].chunk(2, 1)
+    # (as g * sigmoid: 1 + tanh cancels to 0 in 64 bits from about -7 on)
+    h = g * torch.sigmoid(g if act == "silu" else 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)) * u
+    hd = O.value_rows(*O.quantize_rows(h))[:, :128]
+    ref = hd[:, torch.arange(H) % I]
+    # a code may fall the other way (2^-3 of the value, or the smallest step,
+    # 2^-9 of the scale), and the output is rounded to bf16
+    step = h[:, :128].abs().amax(1, keepdim=True).clamp_min(1e-30) / 448 * 2.0 ** -9
+    assert bool(((y - ref).abs() <= (2.0 ** -3 + 2.0 ** -7) * ref.abs() + 1.01 * step).all())
