@@ -385,10 +385,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
   int my_id = p.E;
   float prev = INFINITY;
   int prev_id = -1;
-  // one more round than k where the last kept and the first dropped value
-  // have to be told apart
-  const int rounds = ONLY_LOGITS ? p.k : p.k + 1;
-  for (int j = 0; j < rounds; ++j) {
+  for (int j = 0; j < p.k; ++j) {
     uint32_t best = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) best = max(best, key[i]);
@@ -421,7 +418,23 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
       prev = c;
       prev_id = at;
     }
-    if (lane == j && j < p.k) { my_id = at; my_w = sv; }
+    if (lane == j) { my_id = at; my_w = sv; }
+  }
+  if constexpr (!ONLY_LOGITS) {
+    // is any expert left that may be better than the last one taken? (Not only
+    // the next: behind several equal ones f32 may hide a better one.)
+    uint32_t close = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) close |= (uint32_t)(key[i] > kNegInfKey && prev - order_val(key[i]) <= tol) << i;
+    if (prev_id >= 0 && __any_sync(0xFFFFFFFFu, close)) {
+      const float la = route_logit<DT>(p, row, prev_id), ba = p.bias ? p.bias[prev_id] : 0.0f;
+      bool differs = false;
+      for (; close; close &= close - 1) {
+        const int e = lane * PER + __ffs(close) - 1;
+        differs |= !(route_logit<DT>(p, row, e) == la && (p.bias ? p.bias[e] : 0.0f) == ba);
+      }
+      again |= __any_sync(0xFFFFFFFFu, differs);
+    }
   }
   // scores that f32 holds with fewer bits, or not at all
   const uint32_t used = __ballot_sync(0xFFFFFFFFu, my_id < p.E);

@@ -212,3 +212,21 @@ def test_streams_and_graph():
         x.copy_(y)
         graph.replay()
         assert all(torch.equal(a, c) for a, c in zip(out, route_topk(y, 8, score="sigmoid", bias=b)))
+
+
+@pytest.mark.parametrize("E", [20, 64, 128, 256, 1000])
+def test_a_better_expert_behind_equal_ones(E):
+    """More equal experts than slots, then one whose score is larger by less
+    than f32 holds: it goes first. (A step of f32 at 20 is 2^-19: the sigmoids
+    differ by 4e-15.)"""
+    up = float(np.nextafter(np.float32(20), np.float32(21)))
+    l = torch.full((6, E), 20.0)
+    l[0, E - 1] = l[1, E // 2] = l[2, E - 2] = l[2, E - 3] = up
+    l[3, : E // 2] = up
+    l[4, ::3] = up
+    l = l.cuda()
+    for k in (1, 3, 8):
+        for bias in (torch.zeros(E).cuda(), torch.full((E,), 0.5).cuda()):
+            _, ids = check(l, k, score="sigmoid", bias=bias)
+            assert ids[0, 0] == E - 1 and ids[1, 0] == E // 2 and ids[2, 0] == E - 3
+        check(l, k, score="sigmoid", n_group=4, topk_group=2, group_score="top2")
