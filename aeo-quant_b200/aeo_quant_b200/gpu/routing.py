@@ -42,10 +42,12 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
         scale: factor on the weights.
 
     Returns ``(weights (T, k) float32, ids (T, k) int64)``, experts in
-    descending order of score + bias, equal ones by index. The ids are those
-    of exact arithmetic. A slot for which no expert is left has id E and
-    weight 0 (the expert forwards skip it); a row that holds a NaN (for
-    softmax, or +inf) has NaN weights.
+    descending order of score + bias in 64-bit arithmetic; equal ones by the
+    larger logit, then by the lower index (equal groups by the logit of their
+    best expert), so that a bias that is the same for all changes nothing. A
+    slot for which no expert is left has id E and weight 0 (the expert
+    forwards skip it); a row that holds a NaN (for softmax, or +inf) has NaN
+    weights.
     """
     if logits.ndim != 2:
         raise ValueError(f"logits must be 2D (tokens, experts); got shape {tuple(logits.shape)}")

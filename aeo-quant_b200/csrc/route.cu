@@ -6,18 +6,21 @@
 //   worth(group) = max c, or the sum of its two largest c (a missing second
 //   one counts 0); experts outside the best `topk_group` groups get c = -inf
 //   ids = the k largest c in descending order;  w = s[ids] (/ sum) * scale
-// Equal values go to the lower index. A slot for which no expert is left
+// Equal values go by the larger logit, then by the lower index (equal groups by
+// the logit of their best expert, then by index). A slot for which no expert is left
 // (c = -inf) gets id E and weight 0: the expert forwards skip ids outside
 // [0, E). A row with a NaN logit or choice (softmax: or a +inf logit) gets
 // NaN weights for ids 0..k-1, so that the NaN reaches the layer's output.
 //
-// The ids are those of exact arithmetic. Without a bias both scores rise
+// The ids are those of 64-bit arithmetic. Without a bias both scores rise
 // with the logit, so the choice compares the logits themselves (softmax
 // probabilities of one row, and sigmoids, order as their logits do; group
 // maxima too). With a bias, or with top-2 group sums, the warp compares f32
 // values and notes whether any comparison that decided was closer than
 // their error bound; such a row (about one in a thousand at 256 experts and
-// normal logits) is done again in 64 bits.
+// normal logits) is done again in 64 bits. There sigmoids of all logits from
+// about 37 on are 1, and small scores vanish beside a bias: that equal values
+// go by their logits makes a bias that is the same for all change nothing.
 //
 // Layout: lane L holds the experts L*PER .. L*PER+PER-1, so a row is read
 // with wide loads and the lowest lane that holds a maximum also holds the
@@ -83,23 +86,39 @@ __device__ __forceinline__ float route_logit(const RouteParams& p, int64_t row, 
   return In<DT>::load(reinterpret_cast<const typename In<DT>::T*>(p.logits) + row * p.ld + e);
 }
 
-// Which groups stay: bit g of the result. top1/top2 of the groups come as the
-// (ordered) keys of lane g. `near` is set where a kept and a dropped group
-// are within tol of one another.
-template <class Val>
-__device__ __forceinline__ uint32_t keep_groups(Val worth, int n_group, int topk_group, Val tol, bool& near) {
+// A logit as an ordered key (-0 and +0 are equal).
+template <int DT>
+__device__ __forceinline__ uint32_t route_logit_key(const RouteParams& p, int64_t row, int e) {
+  return order_key(route_logit<DT>(p, row, e) + 0.0f);
+}
+
+// Which groups stay: bit g of the result. Lane g holds group g's worth and, with
+// BY_LOGIT, the key of its best expert's logit. `near` is set where a kept and a
+// dropped group are within tol of one another (in 64 bits: equal).
+template <class Val, bool BY_LOGIT = false>
+__device__ __forceinline__ uint32_t keep_groups(Val worth, int n_group, int topk_group, Val tol, bool& near,
+                                                uint32_t lead = 0) {
   const int lane = threadIdx.x & 31;
   int rank = 0;
   for (int h = 0; h < n_group; ++h) {
     const Val o = __shfl_sync(0xFFFFFFFFu, worth, h);
-    rank += (o > worth) || (o == worth && h < lane);
+    if constexpr (BY_LOGIT) {
+      const uint32_t l = __shfl_sync(0xFFFFFFFFu, lead, h);
+      rank += o > worth || (o == worth && (l > lead || (l == lead && h < lane)));
+    } else {
+      rank += (o > worth) || (o == worth && h < lane);
+    }
   }
   const uint32_t keep = __ballot_sync(0xFFFFFFFFu, lane < n_group && rank < topk_group);
   bool mine = false;
   for (int h = 0; h < n_group; ++h) {
     const Val o = __shfl_sync(0xFFFFFFFFu, worth, h);
-    const Val d = o > worth ? o - worth : worth - o;       // inf - inf is NaN: not near
-    mine |= lane < n_group && (((keep >> h) ^ (keep >> lane)) & 1u) && d <= tol;
+    if constexpr (sizeof(Val) == 8) {
+      mine |= lane < n_group && (((keep >> h) ^ (keep >> lane)) & 1u) && o == worth && worth > -INFINITY;
+    } else {
+      const Val d = o > worth ? o - worth : worth - o;       // inf - inf is NaN: not near
+      mine |= lane < n_group && (((keep >> h) ^ (keep >> lane)) & 1u) && d <= tol;
+    }
   }
   near = __any_sync(0xFFFFFFFFu, mine);
   return keep;
@@ -107,14 +126,17 @@ __device__ __forceinline__ uint32_t keep_groups(Val worth, int n_group, int topk
 
 // One row in 64 bits: the same definition, plainly. Rows come here when f32
 // cannot tell two choices apart, or when every chosen score is so small that
-// f32 has lost it.
-template <int PER, int DT, bool ONLY_LOGITS>
-__device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
+// f32 has lost it. Without BY_LOGIT it stops where two values are equal that
+// the choice may be between, and returns true: the row is then done with it.
+template <int PER, int DT, bool ONLY_LOGITS, bool BY_LOGIT>
+__device__ __noinline__ bool route_row64(const RouteParams& p, int64_t row) {
+  // (with it, small code: few rows come here twice)
+  constexpr int kUnroll = BY_LOGIT ? 1 : PER;
   const int lane = threadIdx.x & 31;
   double s[PER];
   uint64_t key[PER];
   double m = -INFINITY;
-#pragma unroll
+#pragma unroll kUnroll
   for (int i = 0; i < PER; ++i) {
     const int e = lane * PER + i;
     s[i] = e < p.E ? (double)route_logit<DT>(p, row, e) : -INFINITY;
@@ -125,11 +147,11 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
     m = order_val64(warp_max64(order_key64(m)));
     if (m == -INFINITY) m = 0.0;
     double t = 0.0;
-#pragma unroll
+#pragma unroll kUnroll
     for (int i = 0; i < PER; ++i) t += exp(s[i] - m);
     total = warp_sum64(t);
   }
-#pragma unroll
+#pragma unroll kUnroll
   for (int i = 0; i < PER; ++i) {
     const int e = lane * PER + i;
     const double l = s[i];
@@ -144,7 +166,7 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
     const bool whole = S % PER == 0 && (lpg & (lpg - 1)) == 0;
     if (whole) {
       uint64_t a = 0, b = 0;
-#pragma unroll
+#pragma unroll kUnroll
       for (int i = 0; i < PER; ++i) {
         if (key[i] > a) { b = a; a = key[i]; }
         else if (key[i] > b) b = key[i];
@@ -163,7 +185,7 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
     }
     for (int g = 0; g < p.n_group && !whole; ++g) {
       uint64_t a = 0, b = 0;
-#pragma unroll
+#pragma unroll kUnroll
       for (int i = 0; i < PER; ++i) {
         const int e = lane * PER + i;
         if (e >= g * S && e < (g + 1) * S) {
@@ -179,8 +201,30 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
       if (lane == g) worth = v;
     }
     bool near;
-    const uint32_t keep = keep_groups<double>(worth, p.n_group, p.topk_group, 0.0, near);
-#pragma unroll
+    uint32_t lead = 0;
+    if constexpr (BY_LOGIT) {
+      for (int g = 0; g < p.n_group; ++g) {
+        uint64_t a = 0;
+#pragma unroll kUnroll
+        for (int i = 0; i < PER; ++i) {
+          const int e = lane * PER + i;
+          if (e >= g * S && e < (g + 1) * S && key[i] > a) a = key[i];
+        }
+        a = warp_max64(a);
+        uint32_t equal = 0, l = 0;
+#pragma unroll kUnroll
+        for (int i = 0; i < PER; ++i) {
+          const int e = lane * PER + i;
+          equal |= (uint32_t)(e >= g * S && e < (g + 1) * S && key[i] == a) << i;
+        }
+        for (; equal; equal &= equal - 1) l = max(l, route_logit_key<DT>(p, row, lane * PER + __ffs(equal) - 1));
+        l = __reduce_max_sync(0xFFFFFFFFu, l);
+        if (lane == g) lead = l;
+      }
+    }
+    const uint32_t keep = keep_groups<double, BY_LOGIT>(worth, p.n_group, p.topk_group, 0.0, near, lead);
+    if (!BY_LOGIT && !ONLY_LOGITS && near) return true;
+#pragma unroll kUnroll
     for (int i = 0; i < PER; ++i) {
       const int e = lane * PER + i;
       if (e < p.E && !((keep >> (e / S)) & 1u)) key[i] = kNegInfKey64;
@@ -188,25 +232,59 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
   }
   double my_w = 0.0;
   int my_id = p.E;
-  for (int j = 0; j < p.k; ++j) {
+  uint64_t prev = 0;
+  constexpr bool kLook = !BY_LOGIT && !ONLY_LOGITS;
+  for (int j = 0; j < p.k + (int)kLook; ++j) {
     uint64_t best = 0;
-#pragma unroll
+#pragma unroll kUnroll
     for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
     const uint64_t top = warp_max64(best);
     if (top <= kNegInfKey64) break;
-    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+    if constexpr (kLook) {
+      if (top == prev) return true;
+      if (j == p.k) break;
+      prev = top;
+    }
     int at = 0;
     double sv = 0.0;
-    if (lane == src) {
-      bool done = false;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (!done && key[i] == top) {
-          done = true;
-          key[i] = 0;
-          at = lane * PER + i;
-          sv = s[i];
+    int src;
+    if constexpr (BY_LOGIT) {
+      uint32_t equal = 0, mine = 0;      // which of this lane's have that value, their largest logit
+#pragma unroll kUnroll
+      for (int i = 0; i < PER; ++i) equal |= (uint32_t)(key[i] == top) << i;
+      int pick = -1;
+      for (; equal; equal &= equal - 1) {
+        const int i = __ffs(equal) - 1;
+        const uint32_t l = route_logit_key<DT>(p, row, lane * PER + i);
+        if (l > mine) {
+          mine = l;
+          pick = i;
         }
+      }
+      const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, mine);
+      src = __ffs(__ballot_sync(0xFFFFFFFFu, pick >= 0 && mine == most)) - 1;
+      if (lane == src) {
+        at = lane * PER + pick;
+#pragma unroll kUnroll
+        for (int i = 0; i < PER; ++i)
+          if (i == pick) {
+            key[i] = 0;
+            sv = s[i];
+          }
+      }
+    } else {
+      src = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+      if (lane == src) {
+        bool done = false;
+#pragma unroll kUnroll
+        for (int i = 0; i < PER; ++i)
+          if (!done && key[i] == top) {
+            done = true;
+            key[i] = 0;
+            at = lane * PER + i;
+            sv = s[i];
+          }
+      }
     }
     at = __shfl_sync(0xFFFFFFFFu, at, src);
     sv = __shfl_sync(0xFFFFFFFFu, sv, src);
@@ -220,6 +298,7 @@ __device__ __noinline__ void route_row64(const RouteParams& p, int64_t row) {
     p.w[row * p.k + lane] = (float)(my_w * (double)p.scale);
     p.ids[row * p.k + lane] = my_id;
   }
+  return false;
 }
 
 // ONLY_LOGITS: no bias and no top-2 group sums, so logits decide (exactly).
@@ -409,8 +488,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
     sv = __shfl_sync(0xFFFFFFFFu, sv, src);
     if constexpr (!ONLY_LOGITS) {
       const float c = order_val(top);
+      again |= c == INFINITY;              // there may be more of them
       if (prev - c <= tol && prev_id >= 0) {
-        // equal logits and biases are equal in exact arithmetic too
+        // equal logits and biases: equal choice values, to the lower index
         const float la = route_logit<DT>(p, row, at), lb = route_logit<DT>(p, row, prev_id);
         const float ba = p.bias ? p.bias[at] : 0.0f, bb = p.bias ? p.bias[prev_id] : 0.0f;
         again |= !(la == lb && ba == bb);
@@ -441,7 +521,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_topk_kernel(const Rout
   const float sum = warp_sum(my_w);
   again |= used != 0 && sum < 1e-30f;
   if (again) {
-    route_row64<PER, DT, ONLY_LOGITS>(p, row);
+    if (route_row64<PER, DT, ONLY_LOGITS, false>(p, row))
+      if constexpr (!ONLY_LOGITS) route_row64<PER, DT, ONLY_LOGITS, true>(p, row);
     return;
   }
   if (p.renorm) my_w = sum > 0.0f ? my_w / sum : 0.0f;

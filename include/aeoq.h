@@ -490,9 +490,11 @@ AEOQ_API int aeoq_moe_nvfp4_decode_fused_noalloc(const void* hidden, const void*
  * c = -inf where l = -inf. With n_group > 1 the experts form n_group equal
  * runs, of which the topk_group with the largest worth stay. weights (T, k)
  * f32 = s[ids] (divided by their sum if `renormalize`) * scale; ids (T, k)
- * int64: the k largest c in descending order, equal values to the lower
- * index. A slot for which no expert is left has id num_experts and weight 0;
- * a row with a NaN (softmax: or a +inf) has NaN weights and ids 0..k-1.
+ * int64: the k largest c, in 64-bit arithmetic, in descending order; equal
+ * values by the larger logit, then the lower index, equal groups by the logit
+ * of their best expert, then by index. A slot for which no expert is left has
+ * id num_experts and weight 0; a row with a NaN (softmax: or a +inf) has NaN
+ * weights and ids 0..k-1.
  * num_experts <= 1024, k <= 32, n_group <= 32 and dividing num_experts.
  * ------------------------------------------------------------------------ */
 AEOQ_API int aeoq_route_topk(const void* logits, int dtype, int64_t ld, int64_t T, int64_t num_experts, int64_t k,

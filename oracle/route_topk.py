@@ -1,4 +1,8 @@
-"""Expert choice from router logits in 64 bits, row by row (``gpu.routing.route_topk``)."""
+"""Expert choice from router logits in 64 bits, row by row (``gpu.routing.route_topk``).
+
+Choice values that are equal in 64 bits go by the larger logit, then by the
+lower index; groups of equal worth by the logit of their best expert, then by
+the lower index."""
 import numpy as np
 
 
@@ -30,16 +34,17 @@ def route_topk(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, g
             continue
         if n_group > 1:
             g = c.reshape(n_group, -1)
-            worth = []
-            for v in g:
+            worth, lead = [], []
+            for v, r in zip(g, row.reshape(n_group, -1)):
+                lead.append(r[v == v.max()].max())
                 v = np.sort(v)[::-1]
                 second = v[1] if len(v) > 1 and v[1] > -np.inf else 0.0
                 worth.append(v[0] + second if group_score == "top2" else v[0])
-            keep = sorted(range(n_group), key=lambda i: (-worth[i], i))[:topk_group]
+            keep = sorted(range(n_group), key=lambda i: (-worth[i], -lead[i], i))[:topk_group]
             for i in range(n_group):
                 if i not in keep:
                     c[i * (E // n_group):(i + 1) * (E // n_group)] = -np.inf
-        order = [e for e in sorted(range(E), key=lambda e: (-c[e], e)) if c[e] > -np.inf][:k]
+        order = [e for e in sorted(range(E), key=lambda e: (-c[e], -row[e], e)) if c[e] > -np.inf][:k]
         w = s[order]
         if renormalize:
             w = w / w.sum() if w.sum() > 0 else np.zeros_like(w)

@@ -230,3 +230,46 @@ def test_a_better_expert_behind_equal_ones(E):
             _, ids = check(l, k, score="sigmoid", bias=bias)
             assert ids[0, 0] == E - 1 and ids[1, 0] == E // 2 and ids[2, 0] == E - 3
         check(l, k, score="sigmoid", n_group=4, topk_group=2, group_score="top2")
+
+
+def test_saturated_scores_keep_the_order_of_their_logits():
+    """Sigmoids from about 37 on are 1 in 64 bits, and small scores vanish
+    beside a bias: with equal choice values the larger logit goes first, then
+    the lower index, so that a bias that is the same for all changes nothing."""
+    from aeo_quant_b200.gpu.routing import route_topk
+    inf = float("inf")
+    for E, low, high in ((8, 2, 5), (64, 1, 40), (256, 3, 4), (1000, 7, 999)):
+        l = torch.zeros(1, E)
+        l[0, low], l[0, high] = 40.0, 45.0
+        l = l.cuda()
+        rest = next(e for e in range(E) if e not in (low, high))
+        for bias in (None, torch.zeros(E).cuda(), torch.full((E,), 0.25).cuda(), torch.full((E,), inf).cuda()):
+            assert route_topk(l, 3, score="sigmoid", bias=bias)[1].tolist() == [[high, low, rest]]
+    # groups: the better of two saturated ones, and the sums of their two best
+    l = torch.zeros(1, 32)
+    l[0, 3], l[0, 9], l[0, 10] = 40.0, 45.0, -5.0
+    l = l.cuda()
+    for bias in (None, torch.zeros(32).cuda()):
+        kw = dict(score="sigmoid", bias=bias, n_group=4, topk_group=1)
+        assert route_topk(l, 2, **kw)[1].tolist() == [[9, 8]]
+        assert route_topk(l, 2, group_score="top2", **kw)[1].tolist() == [[9, 8]]
+    # equal logits still go by index
+    l = torch.full((2, 64), 50.0).cuda()
+    assert route_topk(l, 4, score="sigmoid", bias=torch.zeros(64).cuda())[1].tolist() == [[0, 1, 2, 3]] * 2
+
+
+@pytest.mark.parametrize("E,n_group,topk_group,k", [(64, 1, 1, 6), (256, 8, 4, 8), (60, 4, 1, 15), (1000, 1, 1, 32),
+                                                    (96, 32, 5, 4)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_bias_that_is_the_same_for_all_changes_no_choice(E, n_group, topk_group, k, score):
+    from aeo_quant_b200.gpu.routing import route_topk
+    l = (torch.randn(500, E, generator=gen(E)) * 30).cuda()
+    l[:20] = l[:20].round()                # equal logits among them
+    kw = dict(score=score, n_group=n_group, topk_group=topk_group)
+    w, ids = route_topk(l, k, **kw)
+    for b in (0.0, 0.1):
+        check(l, k, bias=torch.full((E,), b).cuda(), **kw)
+        w2, ids2 = route_topk(l, k, bias=torch.full((E,), b).cuda(), **kw)
+        assert torch.equal(ids, ids2)
+    check(l, k, bias=(torch.randn(E, generator=gen(1)) * 0.1).cuda(), **kw)
+    check(l, k, bias=torch.zeros(E).cuda(), group_score="top2", **kw)
