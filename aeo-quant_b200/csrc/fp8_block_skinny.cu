@@ -15,6 +15,7 @@
 //
 // The eight warps' sums over K meet in shared memory.
 #include <algorithm>
+#include <cmath>
 
 #include "fp8_block.cuh"
 
@@ -522,11 +523,25 @@ __global__ void __launch_bounds__(kSkThreads, 2) sk_down_kernel(const SkExperts 
   }
 }
 
-// Every pair reads its expert's weights here, the grouped GEMMs read each
-// expert's once but need five launches: at 128 experts, top-8, H = 2816, I =
-// 704 one token takes 23 us (cold L2), 4 tokens 51 against 70, 8 tokens (64
-// pairs) 86 against 90, 16 tokens 158 against 125.
-bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) { return T * k <= 64; }
+// Every pair reads its expert's weights here; the grouped GEMMs read each
+// expert's once for 32 rows, but need five launches. So this form takes up to
+// 64 pairs while what it reads more than once is under 45 MB, the experts in
+// use being as many as with choices that are all equally likely. Measured for
+// 1 to 128 experts, top 1 to 8, 1 to 64 pairs, three weights of H x I from 512
+// x 128 to 4096 x 14336, cold and warm L2: of 316 such layers this takes the
+// slower form by over 10% in five to seven (limits of 30 to 60 MB do worse). In us,
+// here and grouped, cold: H = 2816, I = 704: 128 experts, top-8, one token 23
+// and 43, 6 tokens 70 and 78, 8 tokens 88 and 95 (12 experts' weights, 74 MB,
+// twice); 8 experts, top-2, 4 tokens 27 and 41, 8 tokens 39 and 43, 32 tokens
+// 117 and 43; H = 4096, I = 14336, 8 experts, top-2: one token 102 and 131, two
+// 188 and 174, 32 tokens 2519 and 250.
+constexpr int64_t kSkMaxPairs = 64;
+constexpr double kSkMaxReread = 45e6;
+bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+  if (T > kSkMaxPairs || T * k > kSkMaxPairs) return false;
+  const double used = (double)E * (1.0 - std::pow(std::max(0.0, 1.0 - (double)k / (double)E), (double)T));
+  return ((double)(T * k) - used) * 3.0 * (double)H * (double)I <= kSkMaxReread;
+}
 
 int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt, const float* weights, int64_t k,
                       const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,

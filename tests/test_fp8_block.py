@@ -133,3 +133,23 @@ def test_dequantize_inverts():
     q, s = O.quantize_rows(w[0])
     got = Q.dequantize_fp8_activation_blocks(q.float().to(torch.float8_e4m3fn), s.float())
     assert torch.allclose(got.double(), O.value_rows(q, s), rtol=1e-6)
+
+
+def test_form_of_few_pairs_goes_by_what_is_read_again(lib):
+    """Up to 64 pairs an expert's weights are streamed once per pair, or the
+    pairs are grouped by expert: by the bytes that streaming would read again.
+    The forms differ in their workspace: h alone, against (among others) an
+    f32 output row per pair."""
+    def streams(T, k, E, H, I):
+        n, h = lib.aeoq_moe_fp8_block_workspace_size(T, k, E, H, I), 4 * T * k * I
+        assert n == -(-h // 256) * 256 or n >= 4 * T * k * H
+        return n < 4 * T * k * H
+    for E, k in ((1, 1), (8, 2), (16, 4), (64, 6), (128, 8), (1024, 32)):
+        assert streams(1, k, E, 2816, 704)                 # one token: no expert twice
+        assert not streams(64 // k + 1, k, E, 2816, 704)
+    # a layer of 128 experts: its few pairs are almost all of other experts
+    assert streams(4, 8, 128, 2816, 704) and streams(6, 8, 128, 2816, 704)
+    # few experts: each of them would be read 8, 16, 32 and 64 times
+    assert not any(streams(*c, 2816, 704) for c in ((32, 2, 8), (64, 1, 4), (32, 2, 2), (64, 1, 1)))
+    # of a small layer that costs less than the grouped form's launches
+    assert streams(32, 2, 8, 512, 128) and streams(8, 2, 8, 1024, 256)

@@ -483,3 +483,17 @@ def test_experts_strongly_negative_gates(T, E, act, gain, I):
     # 2^-9 of the scale), and the output is rounded to bf16
     step = h[:, :128].abs().amax(1, keepdim=True).clamp_min(1e-30) / 448 * 2.0 ** -9
     assert bool(((y - ref).abs() <= (2.0 ** -3 + 2.0 ** -7) * ref.abs() + 1.01 * step).all())
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 16, 9, 512, 1024), (1, 40, 32, 256, 832), (2, 40, 32, 272, 128),
+                                       (3, 6, 2, 512, 2048), (1, 8, 2, 144, 3200), (5, 16, 12, 400, 960),
+                                       (1, 1, 1, 64, 1600), (20, 8, 2, 528, 1792), (33, 8, 1, 256, 1344),
+                                       (64, 4, 1, 512, 1088), (32, 2, 2, 1024, 896), (50, 1, 1, 256, 2112)])
+@pytest.mark.parametrize("act", ["silu", "gelu_pytorch_tanh"])
+def test_experts_few_pairs_wide_layers(T, E, k, H, I, act):
+    """Up to 64 pairs: more slots than a CTA has warps, more of I than one
+    round of loads, and layers of few experts that each take many pairs."""
+    gu, gs = weights(E + H, E, 2 * I, H)
+    dw, ds = weights(E + I, E, H, I)
+    check_experts(randn(T, T, H), *routing(T, T, E, k), gu, gs, dw, ds, act)
+    check_experts(randn(T, T, H), *routing(T + 1, T, E, k, 0.2), gu, gs, dw, ds, act)
