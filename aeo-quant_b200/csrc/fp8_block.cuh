@@ -150,6 +150,7 @@ int fb_linear_skinny(const void* x, int dtype, int64_t ldx, int64_t M, const uin
                      int64_t K, const void* bias, void* out, int out_dt, int64_t ldc, uint8_t* q, float* qs,
                      cudaStream_t st);
 bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I);
+int64_t fb_experts_skinny_most(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I);
 int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt, const float* weights, int64_t k,
                       const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,
                       int64_t I, int act, float* h, void* out, cudaStream_t st);

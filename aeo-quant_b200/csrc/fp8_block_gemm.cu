@@ -949,7 +949,11 @@ struct FbExpertsWs {
     hq = take(P * I);
     hs = take(4 * P * fb_blocks(I));
     y = take(4 * P * H);
-    bytes = o;
+    // never less than for fewer tokens, whose h may take more by itself
+    const size_t whole = o;
+    o = 0;
+    take(4 * fb_experts_skinny_most(T, k, E, H, I) * k * I);
+    bytes = std::max(whole, o);
   }
 };
 

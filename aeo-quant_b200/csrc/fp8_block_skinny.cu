@@ -543,6 +543,17 @@ bool fb_experts_skinny_takes(int64_t T, int64_t k, int64_t E, int64_t H, int64_t
   return ((double)(T * k) - used) * 3.0 * (double)H * (double)I <= kSkMaxReread;
 }
 
+// The most tokens up to T that the rule takes (with T it takes all fewer ones:
+// a token adds k pairs and at most k experts in use).
+int64_t fb_experts_skinny_most(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
+  int64_t lo = 0, hi = std::min(T, kSkMaxPairs) + 1;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    (fb_experts_skinny_takes(mid, k, E, H, I) ? lo : hi) = mid;
+  }
+  return lo;
+}
+
 int fb_experts_skinny(const void* hidden, int64_t T, const void* ids, int ids_dt, const float* weights, int64_t k,
                       const uint8_t* gu, const float* gus, const uint8_t* dw, const float* dws, int64_t E, int64_t H,
                       int64_t I, int act, float* h, void* out, cudaStream_t st) {

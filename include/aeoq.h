@@ -556,6 +556,8 @@ AEOQ_API int aeoq_fp8_block_linear(const void* x, int dtype, int64_t ldx, int64_
  * ceil(H/128)) and (E, ceil(H/128), ceil(I/128)) f32; out (T, H) bf16.
  * H % 16 == 0, I % 64 == 0, k <= 32, E <= 1024. All sums are f32, the
  * weighted one over a token's experts too; out is rounded once.
+ * aeoq_moe_fp8_block_workspace_size never falls as T rises: a workspace for
+ * the most tokens serves every call with fewer.
  * ------------------------------------------------------------------------ */
 AEOQ_API size_t aeoq_moe_fp8_block_workspace_size(int64_t T, int64_t top_k, int64_t num_experts, int64_t hidden,
                                                   int64_t inter);

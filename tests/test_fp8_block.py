@@ -153,3 +153,13 @@ def test_form_of_few_pairs_goes_by_what_is_read_again(lib):
     assert not any(streams(*c, 2816, 704) for c in ((32, 2, 8), (64, 1, 4), (32, 2, 2), (64, 1, 1)))
     # of a small layer that costs less than the grouped form's launches
     assert streams(32, 2, 8, 512, 128) and streams(8, 2, 8, 1024, 256)
+
+
+@pytest.mark.parametrize("E,k,H,I", [(8, 2, 4096, 14336), (8, 2, 128, 8192), (1, 1, 16, 4096), (128, 8, 2816, 704),
+                                     (4, 1, 64, 2048), (64, 6, 256, 64), (1024, 32, 512, 1024), (2, 32, 16, 6400)])
+def test_workspace_of_more_tokens_serves_fewer(lib, E, k, H, I):
+    sizes = [lib.aeoq_moe_fp8_block_workspace_size(T, k, E, H, I) for T in range(300)]
+    assert sizes == sorted(sizes)
+    for N, K in ((1408, 2816), (40000, 16)):
+        sizes = [lib.aeoq_fp8_block_linear_workspace_size(M, N, K) for M in range(300)]
+        assert sizes == sorted(sizes)
