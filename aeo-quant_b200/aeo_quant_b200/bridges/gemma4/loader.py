@@ -140,7 +140,9 @@ def quantize_experts_to_fp8_block(model):
     """Replace every bf16 ``Gemma4TextExperts`` in ``model`` by a
     ``Gemma4TextExpertsFP8Block`` holding its block-scaled FP8 quantization
     (``quantize_3d_to_fp8_block``), on the experts' device, one layer at a
-    time. Returns the number of modules converted."""
+    time. Experts whose sizes or activation the kernels do not take are
+    refused before any layer is replaced. Returns the number of modules
+    converted."""
     from ...gpu.quant import quantize_3d_to_fp8_block
     from .modeling_fp8_block import Gemma4TextExpertsFP8Block
 
@@ -148,12 +150,11 @@ def quantize_experts_to_fp8_block(model):
     for _, mod in model.named_modules():
         for child_name, child in mod.named_children():
             if type(child) is modeling_gemma4.Gemma4TextExperts:
-                targets.append((mod, child_name, child, _activation_name(child)))
-    for parent, child_name, old, activation in targets:
-        shape = _ExpertShape(old)
-        shape.hidden_activation = activation
-        with torch.device("meta"):
-            new = Gemma4TextExpertsFP8Block(shape)
+                shape = _ExpertShape(child)
+                shape.hidden_activation = _activation_name(child)
+                with torch.device("meta"):
+                    targets.append((mod, child_name, child, Gemma4TextExpertsFP8Block(shape)))
+    for parent, child_name, old, new in targets:
         for proj in ("gate_up_proj", "down_proj"):
             q, scale = quantize_3d_to_fp8_block(getattr(old, proj).detach())
             setattr(new, proj, torch.nn.Parameter(q, requires_grad=False))

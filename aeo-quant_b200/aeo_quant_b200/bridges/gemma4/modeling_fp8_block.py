@@ -40,6 +40,9 @@ class Gemma4TextExpertsFP8Block(Gemma4TextExperts):
                              f"(one of {sorted(moe_ops._ACTIVATIONS)})")
         self.act_fn = ACT2FN["gelu_pytorch_tanh" if self.activation == "gelu_tanh" else self.activation]
         ne, im, hd = self.num_experts, self.intermediate_dim, self.hidden_dim
+        if hd % 16 or im % 64 or not 1 <= ne <= 1024:
+            raise ValueError(f"hidden_size ({hd}) must be a multiple of 16, moe_intermediate_size ({im}) of 64, "
+                             f"num_experts ({ne}) at most 1024")
         blocks = lambda n: -(-n // 128)  # noqa: E731
         for name, out_dim, in_dim in (("gate_up_proj", 2 * im, hd), ("down_proj", hd, im)):
             setattr(self, name, nn.Parameter(torch.empty(ne, out_dim, in_dim, dtype=torch.float8_e4m3fn),

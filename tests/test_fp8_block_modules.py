@@ -173,3 +173,24 @@ def test_stack_converted_saved_and_loaded(tmp_path):
             ref, tol = O.experts(x.double(), i, w.double(), e.gate_up_proj.double(), e.gate_up_proj_scale.double(),
                                  e.down_proj.double(), e.down_proj_scale.double(), "gelu_pytorch_tanh")
             assert bool(((y.double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("bad", [dict(H=264), dict(I=96), dict(E=1025, H=16, I=64)])
+def test_sizes_that_the_kernels_do_not_take_are_refused_cpu(monkeypatch, bad):
+    """By the module, and by the conversion before any layer is replaced."""
+    from transformers.models.gemma4.modeling_gemma4 import Gemma4TextExperts
+    from aeo_quant_b200.bridges.gemma4 import Gemma4TextExpertsFP8Block, loader
+    from aeo_quant_b200.gpu import quant
+    with pytest.raises(ValueError, match="multiple of 16"):
+        Gemma4TextExpertsFP8Block(config(**bad))
+    monkeypatch.setattr(quant, "quantize_3d_to_fp8_block", lambda w: (
+        w.to(F8), torch.ones(w.shape[0], -(-w.shape[1] // 128), -(-w.shape[2] // 128))))
+    model = nn.Module()
+    model.good, model.bad = Gemma4TextExperts(config()), Gemma4TextExperts(config(**bad))
+    for p in model.parameters():
+        nn.init.zeros_(p)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        loader.quantize_experts_to_fp8_block(model)
+    assert type(model.good) is Gemma4TextExperts and type(model.bad) is Gemma4TextExperts
+    del model.bad
+    assert loader.quantize_experts_to_fp8_block(model) == 1 and type(model.good) is Gemma4TextExpertsFP8Block
