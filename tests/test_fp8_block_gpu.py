@@ -497,3 +497,19 @@ def test_experts_few_pairs_wide_layers(T, E, k, H, I, act):
     dw, ds = weights(E + I, E, H, I)
     check_experts(randn(T, T, H), *routing(T, T, E, k), gu, gs, dw, ds, act)
     check_experts(randn(T, T, H), *routing(T + 1, T, E, k, 0.2), gu, gs, dw, ds, act)
+
+
+@pytest.mark.parametrize("M", [4, 6, 8, 12, 30, 64, 200])
+def test_linear_rows_beside_nan_and_infinite_ones(M):
+    """The rows of a call that also holds NaN and infinite rows have the bits
+    that they have beside finite ones."""
+    from aeo_quant_b200.gpu.fp8_block_matmul import fp8_block_linear
+    w, s = weights(31, 1, 300, 400)
+    x = randn(32, M, 400)
+    want = check_linear(x, w[0], s[0])
+    bad = x.clone()
+    bad[1, 390], bad[2, 3], bad[M - 1] = float("nan"), float("-inf"), float("inf")
+    got = fp8_block_linear(bad, w[0], s[0])
+    keep = torch.ones(M, dtype=torch.bool, device="cuda")
+    keep[1:3] = keep[M - 1] = False
+    assert bool(got[~keep].isnan().all()) and torch.equal(got[keep], want[keep])
