@@ -154,7 +154,7 @@ __device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off
 // against 145).
 template <int kCols>
 __device__ __forceinline__ void fb_store_tile(const FbParams& p, const CUtensorMap& tmO, const FbTile& cur,
-                                              uint8_t* box, const float (&acc)[kCols], int row, int half, bool alive) {
+                                              uint8_t* box, const float (&acc)[kCols], int row, int half) {
   const int64_t n0 = cur.n0 + half * kCols;
 #pragma unroll
   for (int i = 0; i < kCols / 8; ++i) {
@@ -166,7 +166,7 @@ __device__ __forceinline__ void fb_store_tile(const FbParams& p, const CUtensorM
   }
   sm100::fence_proxy_async_smem();
   asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-  if (row == 0 && alive) {
+  if (row == 0) {
 #pragma unroll
     for (int x = 0; x < kCols / 64; ++x)
       if (n0 + 64 * x < p.N)
@@ -185,14 +185,14 @@ __device__ __forceinline__ void fb_store_tile(const FbParams& p, const CUtensorM
 // at a time, so that a store instruction writes four whole lines.
 template <class T, int kCols>
 __device__ __forceinline__ void fb_store_rows(const FbParams& p, const FbTile& cur, uint8_t* box,
-                                              const float (&acc)[kCols], int q, int half, bool alive) {
+                                              const float (&acc)[kCols], int q, int half) {
   constexpr int kPer = 16 / (int)sizeof(T), kRound = 8 * kPer;     // columns per piece, per round
   const int lane = threadIdx.x & 31;
   const int64_t n0 = cur.n0 + half * kCols;
   const bool wide = p.ldc % kPer == 0 && (uintptr_t)p.out % 16 == 0;
   const int sub = lane >> 3, ch = lane & 7;
   T* out = reinterpret_cast<T*>(p.out) + (cur.row0 + 32 * q + sub) * p.ldc + n0 + ch * kPer;
-  const int rows = alive ? cur.rows - 32 * q - sub : 0;            // row 4 j exists if 4 j < rows
+  const int rows = cur.rows - 32 * q - sub;                        // row 4 j exists if 4 j < rows
 #pragma unroll
   for (int x = 0; x < kCols / kRound; ++x) {
     const int64_t left = p.N - n0 - x * kRound - ch * kPer;        // columns from this lane's piece on
@@ -232,7 +232,7 @@ __device__ __forceinline__ void fb_store_rows(const FbParams& p, const FbTile& c
 // both halves where the second exists (`both`). Columns past I count as
 // zeros.
 __device__ __forceinline__ void fb_glu_half(const FbParams& p, const FbTile& cur, float (*amax)[128], bool both,
-                                            float (&acc)[128], int row, int half, bool alive) {
+                                            float (&acc)[128], int row, int half) {
   const int64_t n0 = cur.n0 + 64 * half;
   const int n_ok = (int)min((int64_t)64, p.I - n0);
   const float2 ac = fb_act_of(p.act);
@@ -252,7 +252,7 @@ __device__ __forceinline__ void fb_glu_half(const FbParams& p, const FbTile& cur
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kFbEpiWarps) : "memory");
   }
   const float2 s = fb_scales(__uint_as_float(key));
-  if (row >= cur.rows || !alive) return;
+  if (row >= cur.rows) return;
   if (half == 0) p.hs[(cur.row0 + row) * p.hs_ld + cur.n0 / kFbBlock] = s.y;
   uint8_t* d = p.hq + (cur.row0 + row) * p.hq_ld + n0;
 #pragma unroll
@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
     constexpr int kChunks = kCols / 32;
     uint32_t g = 0;
     // A warp whose wait ran out goes through its remaining tiles without
-    // waiting or storing: the other warps count on it at the barriers below.
+    // waiting, as the other warps count on it at the barriers below, and
+    // stores NaN, so that nobody takes what was there before for the result.
     bool alive = true;
     FbTile ti{};
     const float *sa = p.sa, *sw0 = p.sw, *sw1 = p.sw;
@@ -460,6 +461,10 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
           for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), cs, acc[32 * c + i]);
         }
       }
+      if (!alive) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[i] = __int_as_float(0x7FC00000);
+      }
       if (t + (int)gridDim.x < total) open_tile(t + gridDim.x);   // its loads run under the stores
       if constexpr (EPI == kFbStore) {
         if (p.bias) {
@@ -471,11 +476,11 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_gemm_kernel(const __g
         uint8_t* box = base + L::kStages * L::kStage + half * (128 * kCols * 2);
         if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-        if (p.out_tma) fb_store_tile(p, tmO, cur, box, acc, row, half, alive);
-        else if (p.out_dt == AEOQ_BF16) fb_store_rows<__nv_bfloat16>(p, cur, box + q * 4096, acc, q, half, alive);
-        else fb_store_rows<float>(p, cur, box + q * 4096, acc, q, half, alive);
+        if (p.out_tma) fb_store_tile(p, tmO, cur, box, acc, row, half);
+        else if (p.out_dt == AEOQ_BF16) fb_store_rows<__nv_bfloat16>(p, cur, box + q * 4096, acc, q, half);
+        else fb_store_rows<float>(p, cur, box + q * 4096, acc, q, half);
       } else {
-        fb_glu_half(p, cur, sh->amax, both, acc, row, half, alive);
+        fb_glu_half(p, cur, sh->amax, both, acc, row, half);
       }
     }
   }
@@ -688,7 +693,11 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
           w1 = __ldg(sw1 + kb + 1);
         }
         if (alive) alive = sm100::mbar_wait(&sh->acc_full[b], bph, p.err, 85);
-        if (!alive) continue;
+        if (!alive) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[0][j] = acc[1][j] = __int_as_float(0x7FC00000);
+          continue;
+        }
         sm100::tc_fence_after();
         const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + b * 64 + tok0;
         float r0[16], r1[16];
@@ -707,7 +716,6 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
       if constexpr (EPI == kFbStore) {
         // 32 lanes store 128 consecutive bytes of a token's row
         float* d = reinterpret_cast<float*>(p.out) + (ti.row0 + tok0) * p.ldc + ti.n0 + f;
-        if (!alive) continue;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           if (j >= n_tok) break;
@@ -730,7 +738,6 @@ __global__ void __launch_bounds__(kFbThreads, 1) fp8_block_few_kernel(const __gr
         for (int i = 0; i < 4; ++i) k = max(k, sh->amax[half][i][lane & 15]);
         asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
         const float2 s = fb_scales(__uint_as_float(k));      // of token lane & 15
-        if (!alive) continue;
         if (q == 0 && lane < n_tok) p.hs[(ti.row0 + tok0 + lane) * p.hs_ld + ti.n0 / kFbBlock] = s.y;
         uint8_t* d = p.hq + (ti.row0 + tok0) * p.hq_ld + ti.n0 + f;
 #pragma unroll

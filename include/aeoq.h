@@ -527,8 +527,9 @@ AEOQ_API int aeoq_fp8_block_quantize_weights(const void* x, int dtype, int64_t n
  * ceil(K/128)) and sw (ceil(N/128), ceil(K/128)) f32; bias N bf16 values or
  * null; out BF16 or F32 with a row stride of ldc elements. K % 16 == 0; M
  * and N are free. err_word (a device int, or null) is set non-zero if a
- * bounded wait runs out (never expected). No counterpart in the reference,
- * whose FP8 linear has one scale per row (aeoq_fp8_gemm).
+ * bounded wait runs out (never expected); what the waiting warps would have
+ * stored is then NaN. No counterpart in the reference, whose FP8 linear has one
+ * scale per row (aeoq_fp8_gemm).
  *
  * aeoq_fp8_block_linear quantizes its input first
  * (aeoq_fp8_block_quantize_rows; x BF16/F16/F32, row stride ldx) into the
