@@ -513,3 +513,11 @@ def test_linear_rows_beside_nan_and_infinite_ones(M):
     keep = torch.ones(M, dtype=torch.bool, device="cuda")
     keep[1:3] = keep[M - 1] = False
     assert bool(got[~keep].isnan().all()) and torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("N", [1, 8, 16, 24, 63, 72, 136, 264])
+@pytest.mark.parametrize("M,K", [(64, 16), (130, 144), (400, 128)])
+def test_linear_narrow_outputs(M, N, K):
+    """Outputs narrower than a store's box of 64 columns, or a little wider."""
+    w, s = weights(N + K, 1, N, K)
+    check_linear(randn(M, M, K), w[0], s[0])
