@@ -5,9 +5,10 @@ weights, beside ``Gemma4TextExpertsFP8`` (one scale per output row) and
 Buffers: ``gate_up_proj`` (E, 2I, H) and ``down_proj`` (E, H, I)
 float8_e4m3fn Parameters, ``gate_up_proj_scale`` (E, ceil(2I/128),
 ceil(H/128)) and ``down_proj_scale`` (E, ceil(H/128), ceil(I/128)) float32,
-one scale per 128 x 128 block. Forward signature and routing as the other
-expert modules (HF transformers 5.5.0 ``Gemma4TextExperts``); any router's
-``(top_k_index, top_k_weights)`` will do, ``gpu.routing.route_topk``'s
+one scale per 128 x 128 block of the fused matrix (where I is not a multiple
+of 128 a block holds gate and up rows). Forward signature and routing as the
+other expert modules (HF transformers 5.5.0 ``Gemma4TextExperts``); any
+router's ``(top_k_index, top_k_weights)`` will do, ``gpu.routing.route_topk``'s
 among them.
 """
 from __future__ import annotations

@@ -140,9 +140,8 @@ __device__ __forceinline__ FbTile fb_tile(const FbParams& p, const int* tile_off
 }
 
 // ---------------------------------------------------------------- epilogues
-// One thread's row of a tile's column half, as the two GEMM kernels below
-// share them. `row` is the thread's row in its 128-row tile; four warps hold
-// one half.
+// One thread's row of a tile's column half. `row` is the thread's row in its
+// 128-row tile; four warps hold one half.
 
 // Store of a whole 128-row tile's kCols bf16 columns from cur.n0 + kCols *
 // half on: through shared memory (a thread's row in pieces of 16 bytes, placed
