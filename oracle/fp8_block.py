@@ -119,7 +119,7 @@ def experts(x, ids, weights, guq, gus, dwq, dws, act):
             dhd[:, lo:lo + B] = (torch.maximum((e4m3(p + dp) - q).abs(), (e4m3(p - dp) - q).abs()) + q.abs() * r) * s
         dw = value_blocks(dwq[e], dws[e])
         y, dy = product(hd, dw)
-        dy = dy + dhd @ dw.abs().T + BF16 * y.abs()
+        dy = dy + dhd @ dw.abs().T
         w = weights[t, j][:, None]
         out.index_add_(0, t, w * y)
         tol.index_add_(0, t, w.abs() * (dy + (ids.shape[1] + 1) * U * y.abs()))
